@@ -373,6 +373,65 @@ int raftcorr_alt_prepare(const float* fmap1, const float* fmap2, int B, int C, i
 int raftcorr_alt_features_bwd(const float* d1, const float* const* d2_levels, int B, int C, int H, int W, int num_levels,
                               float* dfmap1, float* dfmap2, void* stream);
 
+/* ---- around the correlation block: the encoders' norms and the optimizer step --------------------------------------
+ * Element types of the calls below. */
+#define RAFTCORR_DTYPE_FP32 0
+#define RAFTCORR_DTYPE_FP16 1
+#define RAFTCORR_DTYPE_BF16 2
+
+/* Group normalisation with an activation, channels last (replaces nn.GroupNorm / nn.InstanceNorm2d + F.relu of
+ * core/extractor_origin.py:12-55,119-170: instance norm = one channel a group, without weights).  x: N samples of P rows of C
+ * channels, element (n, p, c) at x[n * x_batch + p * x_row + c]; groups neighbouring channels share mean and (biased) variance:
+ *   y = act((x - mean) * rstd * weight[c] + bias[c]),  rstd = 1 / sqrt(var + eps)
+ *   weight, bias  (C) float32, each may be NULL (1 and 0).     y: (N, P, C) dense, type of x.
+ *   stats         (N, groups, 2) float32: mean and rstd, always written; the backward call reads it.
+ *   workspace     raftcorr_group_norm_workspace_bytes(N, C, groups) bytes, 16-byte aligned, contents don't-care.
+ * Backward: dy as x (strides of its own), dx (N, P, C) dense or NULL, dweight / dbias (C) float32 or NULL, all overwritten.
+ * relu'(0) = 0.  Statistics and sums are float32; no atomics, the same bits on every call.  x, dy, y, dx need no more than their
+ * element's alignment.  Any C, groups that divide it, P, N >= 1; row stride >= C unless P == 1.
+ * RAFTCORR_EUNSUPPORTED beyond 2^24 - 1 workgroups (N, N * groups / 4 or C / 4 of that order). */
+#define RAFTCORR_ACT_NONE 0
+#define RAFTCORR_ACT_RELU 1
+#define RAFTCORR_ACT_SILU 2
+int64_t raftcorr_group_norm_workspace_bytes(int N, int C, int groups);
+int raftcorr_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int groups,
+                            const float* weight, const float* bias, double eps, int act, void* y, float* stats,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+int raftcorr_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t dy_batch, int64_t dy_row,
+                            int dtype, int N, int64_t P, int C, int groups, const float* weight, const float* bias, int act,
+                            const float* stats, void* dx, float* dweight, float* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One AdamW step of many tensors (replaces torch.optim.AdamW + clip_grad_norm_ of core/train_origin.py:84-95,210-216):
+ *   c = min(1, max_norm / (|g| + 1e-6));  m = beta1 m + (1 - beta1) c g;  v = beta2 v + (1 - beta2) (c g)^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * params, grads: HOST arrays of count DEVICE pointers, numels[i] >= 1 values of `dtype` each (FP32 or BF16; bfloat16 parameters
+ * are rounded stochastically).  The state of a bucket of tensors lies in flat buffers; tensor i's starts at value offsets[i], a
+ * multiple of RAFTCORR_ADAMW_TILE, and fills up whole tiles (the rest of the last one stays zero); no two tensors share a tile.
+ *   state_bits 32  exp_avg, exp_avg_sq float32; exponents NULL.
+ *   state_bits 8   exp_avg, exp_avg_sq one byte a value, exp_avg_exp, exp_avg_sq_exp one byte for RAFTCORR_ADAMW_BLOCK values
+ *                  (csrc/adamw.hip has the format); rounded stochastically from (seed, step, position) alone.
+ *   steps          float32, steps[slots[i]] counts tensor i's steps (incremented); scale: float32 scratch, 2 values a slot, each slot
+ *                  of a call once.
+ *   lr_device      NULL, or a device float32 that replaces lr (a captured graph then follows it).
+ * Clipping: raftcorr_adamw_norm leaves raftcorr_adamw_norm_partials(numels, count) float64 sums of squares in `partial`; the sums
+ * of all tensors that share the norm stand one behind the other (`partials` of them) when raftcorr_adamw_step is called, which
+ * writes the norm to `norm` (float32) and the coefficient to `clip` (float64).  partials == 0: no clipping, these may be NULL.
+ * Gradients stay as they are.  Two calls give the same bits.
+ * raftcorr_adamw_decode writes 8-bit moments as numbers (FP32, or BF16, which holds the codes' four digits exactly from 2^-126 up). */
+#define RAFTCORR_ADAMW_TILE  512
+#define RAFTCORR_ADAMW_BLOCK 64
+int64_t raftcorr_adamw_norm_partials(const int64_t* numels, int count);
+int raftcorr_adamw_norm(const void* const* grads, const int64_t* numels, int count, int dtype, double* partial, void* stream);
+int raftcorr_adamw_step(void* const* params, const void* const* grads, const int64_t* numels, const int64_t* offsets,
+                        const int32_t* slots, int count, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,
+                        uint8_t* exp_avg_exp, uint8_t* exp_avg_sq_exp, float* steps, float* scale,
+                        double lr, const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                        uint32_t seed, const double* partial, int partials, double max_norm, double* clip, float* norm,
+                        void* stream);
+int raftcorr_adamw_decode(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_exp, const uint8_t* exp_avg_sq_exp,
+                          int64_t count, int dtype, void* m, void* v, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,11 +13,15 @@ LIB_PATH = os.path.join(_HERE, "libraftcorr.so")
 MAX_LEVELS = 8
 PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2, "fp16x2": 3}          # RAFTCORR_PREC_*
 VOLUMES = {"fp32": 0, "fp16": 1, "bf16": 2}                              # RAFTCORR_VOL_*
+DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}     # RAFTCORR_DTYPE_*, by str(tensor.dtype)
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}                          # RAFTCORR_ACT_*
+ADAMW_TILE, ADAMW_BLOCK = 512, 64                                        # RAFTCORR_ADAMW_*
 MODE_FORK = 0
 MODE_CANONICAL = 1
 
 _c_fp = ctypes.c_void_p          # device pointers travel as plain addresses
 _c_int = ctypes.c_int
+_c_i64 = ctypes.c_int64
 
 # name -> argtypes; mirrors include/raftcorr.h one to one
 _SIGNATURES = {
@@ -89,6 +93,16 @@ _SIGNATURES = {
                                                               ctypes.c_void_p], _c_int),
     "raftcorr_alt_features_bwd": ([_c_fp, ctypes.POINTER(ctypes.c_void_p)] + [_c_int] * 5 + [_c_fp, _c_fp, ctypes.c_void_p],
                                   _c_int),
+    "raftcorr_group_norm_workspace_bytes": ([_c_int] * 3, ctypes.c_int64),
+    "raftcorr_group_norm_fwd": ([_c_fp, _c_i64, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_fp, _c_fp, ctypes.c_double, _c_int,
+                                 _c_fp, _c_fp, _c_fp, _c_i64, ctypes.c_void_p], _c_int),
+    "raftcorr_group_norm_bwd": ([_c_fp, _c_i64, _c_i64, _c_fp, _c_i64, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_int, _c_fp, _c_fp,
+                                 _c_int] + [_c_fp] * 5 + [_c_i64, ctypes.c_void_p], _c_int),
+    "raftcorr_adamw_norm_partials": ([_c_fp, _c_int], _c_i64),
+    "raftcorr_adamw_norm": ([_c_fp, _c_fp, _c_int, _c_int, _c_fp, ctypes.c_void_p], _c_int),
+    "raftcorr_adamw_step": ([_c_fp] * 5 + [_c_int] * 3 + [_c_fp] * 6 + [ctypes.c_double, _c_fp] + [ctypes.c_double] * 4 +
+                            [ctypes.c_uint32, _c_fp, _c_int, ctypes.c_double, _c_fp, _c_fp, ctypes.c_void_p], _c_int),
+    "raftcorr_adamw_decode": ([_c_fp] * 4 + [_c_i64, _c_int, _c_fp, _c_fp, ctypes.c_void_p], _c_int),
 }
 
 EXPORTS = tuple(_SIGNATURES)

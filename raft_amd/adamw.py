@@ -1,0 +1,302 @@
+"""The optimizer step of RAFT's training recipe -- AdamW behind clip_grad_norm_ (core/train_origin.py:84-95,210-216) -- over all
+tensors of a model in a few launches, with moments in 32 or in 8 bits, backed by libraftcorr.so (C ABI in include/raftcorr.h).
+
+PyTorch is used for device memory, streams and the optimizer's bookkeeping only; there is no fallback path.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .corr import _guard, _stream
+
+__all__ = ["AdamW"]
+
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _dense(p):
+    """Whether the tensor's values fill one stretch of memory without gaps or overlaps, in whatever order."""
+    if p.is_contiguous():
+        return True
+    want = 1
+    for s, n in sorted((s, n) for n, s in zip(p.shape, p.stride()) if n > 1):
+        if s != want:
+            return False
+        want *= n
+    return True
+
+
+def _order(t):
+    """The strides that say where the values lie (those of axes of one value do not)."""
+    return [s for n, s in zip(t.shape, t.stride()) if n > 1]
+
+
+class _Bucket:
+    """The parameters of one group that share device and type, and their state in flat buffers: parameter i's moments start at
+    value offsets[i], a multiple of the tile, in the order of the parameter's own memory."""
+
+    def __init__(self, params, bits, index):
+        self.params, self.bits, self.index = params, bits, index
+        self.device, self.dtype = params[0].device, params[0].dtype
+        self.numels = [p.numel() for p in params]
+        self.strides = [p.stride() for p in params]
+        self.offsets, total = [], 0
+        for n in self.numels:
+            self.offsets.append(total)
+            total += (n + _lib.ADAMW_TILE - 1) // _lib.ADAMW_TILE * _lib.ADAMW_TILE
+        self.total = total
+        kind = torch.float32 if bits == 32 else torch.uint8
+        self.m, self.v = (torch.zeros(total, dtype=kind, device=self.device) for _ in range(2))
+        blocks = 0 if bits == 32 else total // _lib.ADAMW_BLOCK
+        self.me, self.ve = (torch.zeros(blocks, dtype=torch.uint8, device=self.device) for _ in range(2))
+        self.steps = torch.zeros(len(params), dtype=torch.float32, device=self.device)
+        self.host = {}                                       # host arrays of a set of present gradients
+
+    def views(self, i):
+        """The state of parameter i as it stands in the optimizer's state."""
+        p, at = self.params[i], self.offsets[i]
+        out = {"step": self.steps[i]}
+        for name, flat in (("exp_avg", self.m), ("exp_avg_sq", self.v)):
+            out[name] = flat.as_strided(p.shape, p.stride(), at)
+        if self.bits == 8:
+            first, last = at // _lib.ADAMW_BLOCK, (at + self.numels[i] + _lib.ADAMW_BLOCK - 1) // _lib.ADAMW_BLOCK
+            out["exp_avg_exponent"], out["exp_avg_sq_exponent"] = self.me[first:last], self.ve[first:last]
+        return out
+
+    def arrays(self, present):
+        """numels, offsets, slots of the parameters `present` (a tuple of indices) as host arrays."""
+        got = self.host.get(present)
+        if got is None:
+            if len(self.host) > 8:
+                self.host.clear()
+            n = len(present)
+            got = self.host[present] = ((ctypes.c_int64 * n)(*[self.numels[i] for i in present]),
+                                        (ctypes.c_int64 * n)(*[self.offsets[i] for i in present]), (ctypes.c_int32 * n)(*present))
+        return got
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW (without amsgrad and maximize) with the clipping by the gradients' global norm inside the step.
+
+    state_bits  32, or 8: each moment in one byte and one exponent byte for 64 of them (include/raftcorr.h); coded with
+                stochastic rounding whose random bits come from (seed, step, position) alone, so a run repeats bit by bit.
+    max_norm    None, or the bound on the 2-norm over all gradients of the optimizer.  The gradients themselves stay as they
+                are; the norm of the last step is in `grad_norm` (a device tensor).
+    lr          a number, or a float32 tensor on the parameters' device, which a captured step reads anew at each replay.
+
+    Parameters: CUDA, float32 or bfloat16 (rounded stochastically; no 32-bit copy is kept), in one stretch of memory.
+    Gradients: of the parameters' type; parameters without one are passed over.  A step can be captured into a HIP graph once
+    one step has been taken; numbers among its options stay what they were.  `state` holds views ("step", "exp_avg", "exp_avg_sq", with 8 bits their codes and exponents) into
+    one buffer a bucket of parameters (write into them; another tensor put in their place is not seen); torch.optim.AdamW's state_dict can be loaded with state_bits=32 and the other way round.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError(f"max_norm must be positive or None, got {max_norm}")
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, max_norm=max_norm, seed=int(seed))
+        self._buckets = None
+        self.grad_norm = None
+        super().__init__(params, defaults)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._buckets, self.grad_norm = None, None
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            _options(group)
+            if group["state_bits"] != self.defaults["state_bits"] or group["max_norm"] != self.defaults["max_norm"]:
+                raise ValueError("state_bits and max_norm hold for the whole optimizer")
+            for p in group["params"]:
+                if p.dtype not in _DTYPES:
+                    raise ValueError(f"parameters must be float32 or bfloat16, got {p.dtype}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+        self._buckets = None                                 # rebuilt around the state there is
+
+    # -- state ------------------------------------------------------------------------------------------------------
+
+    def _ready(self):
+        """The buckets, made on the first call and after a state was loaded or emptied."""
+        if self._buckets is not None and len(self.state) == self._held:
+            return self._buckets
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: take one step before a step is captured (the state is made by the first one)")
+        bits, made = self.defaults["state_bits"], []
+        for group in self.param_groups:
+            by_kind = {}
+            for p in group["params"]:
+                if not p.is_cuda:
+                    raise RuntimeError("parameter must be a CUDA tensor")
+                if p.dtype not in _DTYPES:
+                    raise RuntimeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
+                if not _dense(p):
+                    raise RuntimeError(f"parameter of shape {tuple(p.shape)} and strides {p.stride()} does not lie in one stretch of memory")
+                if p.numel():
+                    by_kind.setdefault((p.device, p.dtype), []).append(p)
+            made.append([])
+            for params in by_kind.values():
+                made[-1].append(_Bucket(params, bits, sum(map(len, made))))
+        for buckets in made:
+            for b in buckets:
+                for i, p in enumerate(b.params):
+                    views, old = b.views(i), self.state.get(p)
+                    if old:
+                        _adopt(views, old, bits)
+                    self.state[p] = views
+        self._buckets, self._held = made, len(self.state)
+        return made
+
+    def load_state_dict(self, state_dict):
+        """Takes the values as they are: the base class would cast them to the parameter's type."""
+        for old in state_dict["state"].values():
+            if old:
+                _adopt(None, old, self.defaults["state_bits"])          # refused before anything is taken over
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise RuntimeError("the loaded state is one of amsgrad or maximize")
+        super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            _options(group)
+            group["state_bits"], group["max_norm"] = self.defaults["state_bits"], self.defaults["max_norm"]
+            group.setdefault("seed", self.defaults["seed"])
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            old = state_dict["state"].get(i)
+            if old:
+                self.state[p] = {k: v.detach().clone() if torch.is_tensor(v) else v for k, v in old.items()}
+        self._buckets = None
+        if params and all(p.is_cuda for p in params):
+            self._ready()
+
+    def packed_moments(self, dtype=None):
+        """[(first, second moments)] of each bucket (a group's parameters of one device and type) as flat tensors, laid out as
+        packed_layout says.  32 bits: the state itself, or a copy in `dtype`.  8 bits: decoded to float32 or bfloat16 (which holds
+        the codes' values exactly from 2^-126 up)."""
+        out = []
+        for b in (b for buckets in self._ready() for b in buckets):
+            if b.bits == 32:
+                out.append((b.m, b.v) if dtype is None else (b.m.to(dtype), b.v.to(dtype)))
+                continue
+            kind = torch.float32 if dtype is None else dtype
+            if kind not in _DTYPES:
+                raise RuntimeError(f"8-bit moments are decoded to float32 or bfloat16, not {kind}")
+            m, v = (torch.empty(b.total, dtype=kind, device=b.device) for _ in range(2))
+            with _guard(m):
+                _lib.check(_lib.load().raftcorr_adamw_decode(b.m.data_ptr(), b.v.data_ptr(), b.me.data_ptr(), b.ve.data_ptr(), b.total,
+                                                             _lib.DTYPES[str(kind)], m.data_ptr(), v.data_ptr(), _stream(m)), "adamw_decode")
+            out.append((m, v))
+        return out
+
+    def packed_layout(self):
+        """[[(parameter, offset)]] of each bucket: where a parameter's moments start in packed_moments (values, a multiple of 512;
+        the gaps are zero).  They follow the order of the parameter's memory."""
+        return [list(zip(b.params, b.offsets)) for buckets in self._ready() for b in buckets]
+
+    # -- step -------------------------------------------------------------------------------------------------------
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = [(group, b) + _gather(b) for group, buckets in zip(self.param_groups, self._ready()) for b in buckets]
+        work = [w for w in work if w[2]]
+        max_norm = self.defaults["max_norm"]
+        if not work:
+            self.grad_norm = None if max_norm is None else torch.zeros(())
+            return loss
+        lib = _lib.load()
+        partial, partials, pieces = None, 0, []
+        if max_norm is not None:
+            if len({b.device for _, b, *_ in work}) > 1:
+                raise RuntimeError("max_norm: the parameters are on more than one device")
+            pieces = [lib.raftcorr_adamw_norm_partials(arrays[0], len(present)) for _, _, present, arrays, *_ in work]
+            partials = sum(pieces)
+            first = work[0][1]
+            partial = torch.empty(partials + 1, dtype=torch.float64, device=first.device)      # the last one: the coefficient
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=first.device)
+            at = partial.data_ptr()
+            for (_, b, present, arrays, _, grads, _), n in zip(work, pieces):
+                with _guard(partial):
+                    _lib.check(lib.raftcorr_adamw_norm(grads, arrays[0], len(present), _lib.DTYPES[str(b.dtype)], at, _stream(partial)),
+                               "adamw_norm")
+                at += 8 * n
+        for group, b, present, (numels, offsets, slots), params, grads, keep in work:
+            lr, (b1, b2) = group["lr"], group["betas"]
+            on_device = torch.is_tensor(lr) and lr.is_cuda
+            if on_device and lr.device != b.device:
+                raise RuntimeError(f"lr is on {lr.device}, expected {b.device}")
+            scale = torch.empty(2 * len(b.params), dtype=torch.float32, device=b.device)
+            with _guard(scale):
+                _lib.check(lib.raftcorr_adamw_step(
+                    params, grads, numels, offsets, slots, len(present), _lib.DTYPES[str(b.dtype)], b.bits, b.m.data_ptr(), b.v.data_ptr(),
+                    b.me.data_ptr() if b.bits == 8 else None, b.ve.data_ptr() if b.bits == 8 else None, b.steps.data_ptr(), scale.data_ptr(),
+                    0.0 if on_device else float(lr), lr.data_ptr() if on_device else None, b1, b2, group["eps"], group["weight_decay"],
+                    (group["seed"] + 7919 * b.index) & 0xFFFFFFFF, partial.data_ptr() if partials else None, partials, max_norm or 0.0,
+                    partial.data_ptr() + 8 * partials if partials else None, self.grad_norm.data_ptr() if partials else None,
+                    _stream(scale)), "adamw_step")
+        return loss
+
+
+def _options(group):
+    lr, betas, eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
+    if torch.is_tensor(lr):
+        if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
+            raise ValueError(f"lr must be a number or one float32 value, got {lr.dtype} {tuple(lr.shape)}")
+    elif not lr >= 0:
+        raise ValueError(f"lr = {lr}")
+    if not (len(betas) == 2 and all(0 <= b < 1 for b in betas)):
+        raise ValueError(f"betas = {betas}")
+    if not eps >= 0 or not decay >= 0:
+        raise ValueError(f"eps = {eps}, weight_decay = {decay}")
+
+
+def _adopt(views, old, bits):
+    """The values of a parameter's loaded state into the buffers (views: a bucket's; None: only look whether they fit)."""
+    names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exponent", "exp_avg_sq_exponent"] if bits == 8 else [])
+    held = 8 if "exp_avg_exponent" in old else 32
+    if held != bits or any(k not in old for k in names):
+        raise RuntimeError(f"the loaded state holds {held}-bit moments, this optimizer keeps {bits}-bit ones")
+    if views is None:
+        return
+    for name in names:
+        if old[name].shape != views[name].shape:
+            raise RuntimeError(f"the loaded {name} has shape {tuple(old[name].shape)}, expected {tuple(views[name].shape)}")
+        if bits == 8 and _order(old[name]) != _order(views[name]):
+            raise RuntimeError(f"the loaded {name} has another memory order than the parameter: its blocks of 8-bit values differ")
+        views[name].copy_(old[name])
+    views["step"].fill_(float(old["step"]))
+
+
+def _gather(b):
+    """(indices of the parameters with a gradient, their host arrays, parameter and gradient addresses, what must stay alive)."""
+    present, ps, gs, keep = [], [], [], []
+    for i, p in enumerate(b.params):
+        g = p.grad
+        if g is None:
+            continue
+        if g.dtype != b.dtype or g.device != b.device or g.layout != torch.strided:
+            raise RuntimeError(f"gradient is {g.dtype}, {g.layout} on {g.device}, expected a dense {b.dtype} on {b.device}")
+        if p.dtype != b.dtype or p.device != b.device or p.numel() != b.numels[i]:
+            raise RuntimeError("a parameter's type, device or size has changed since the state was made")
+        strides = p.stride()
+        if strides != b.strides[i] and [s for n, s in zip(p.shape, b.strides[i]) if n > 1] != _order(p):
+            raise RuntimeError("a parameter's memory order has changed since the state was made")
+        if g.stride() != strides and _order(g) != _order(p):
+            g = torch.empty_like(p).copy_(g)                     # the order of the parameter's memory
+            keep.append(g)
+        present.append(i)
+        ps.append(p.data_ptr())
+        gs.append(g.data_ptr())
+    n = len(ps)
+    present = tuple(present)
+    return present, b.arrays(present) if n else None, (ctypes.c_void_p * n)(*ps), (ctypes.c_void_p * n)(*gs), keep

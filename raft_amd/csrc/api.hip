@@ -574,4 +574,118 @@ int raftcorr_alt_features_bwd(const float* d1, const float* const* d2_levels, in
     return launch_alt_features_bwd(d1, d2_levels, B, C, H, W, num_levels, dfmap1, dfmap2, (hipStream_t)stream);
 }
 
+// ---- group norm, AdamW ----------------------------------------------------------------------------------------------
+
+static const int64_t kMostBlocks = (1 << 24) - 1;      // workgroups of 256 that one launch takes
+
+static int check_group_norm(const char* who, int dtype, int N, int64_t P, int C, int groups, int act, int64_t row, int64_t workspace_bytes,
+                            const void* workspace)
+{
+    if (dtype < RAFTCORR_DTYPE_FP32 || dtype > RAFTCORR_DTYPE_BF16) return fail(RAFTCORR_EINVAL, "%s: dtype = %d", who, dtype);
+    if (act < RAFTCORR_ACT_NONE || act > RAFTCORR_ACT_SILU) return fail(RAFTCORR_EINVAL, "%s: act = %d", who, act);
+    if (N < 1 || P < 1 || C < 1) return fail(RAFTCORR_EINVAL, "%s: N, P, C must be positive (got %d, %lld, %d)", who, N, (long long)P, C);
+    if (groups < 1 || C % groups) return fail(RAFTCORR_EINVAL, "%s: %d channels in %d groups", who, C, groups);
+    if (P > 1 && row < C) return fail(RAFTCORR_EINVAL, "%s: rows of %d channels overlap (stride %lld)", who, C, (long long)row);
+    if (C > 1 << 20 || P > 1LL << 40 || (int64_t)N * ((C + 255) / 256) > kMostBlocks || (int64_t)N * groups / 4 + C / 4 + 1 > kMostBlocks)
+        return fail(RAFTCORR_EUNSUPPORTED, "%s: N = %d, P = %lld, C = %d too large", who, N, (long long)P, C);
+    if (!workspace || workspace_bytes < (int64_t)group_norm_workspace_bytes(N, C, groups))
+        return fail(RAFTCORR_EINVAL, "%s: workspace of %lld bytes, need %lld", who, (long long)workspace_bytes,
+                    (long long)group_norm_workspace_bytes(N, C, groups));
+    return RAFTCORR_OK;
+}
+
+int64_t raftcorr_group_norm_workspace_bytes(int N, int C, int groups)
+{
+    if (N < 1 || C < 1 || groups < 1 || C % groups) return 0;
+    return (int64_t)group_norm_workspace_bytes(N, C, groups);
+}
+
+int raftcorr_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int groups,
+                            const float* weight, const float* bias, double eps, int act, void* y, float* stats,
+                            void* workspace, int64_t workspace_bytes, void* stream)
+{
+    const int rc = check_group_norm("group_norm_fwd", dtype, N, P, C, groups, act, x_row, workspace_bytes, workspace);
+    if (rc) return rc;
+    if (!x || !y || !stats) return fail(RAFTCORR_EINVAL, "group_norm_fwd: null pointer");
+    if (!(eps >= 0.0)) return fail(RAFTCORR_EINVAL, "group_norm_fwd: eps = %g", eps);
+    return launch_group_norm_fwd(x, x_batch, x_row, dtype, N, P, C, groups, weight, bias, (float)eps, act, y, stats, workspace, (hipStream_t)stream);
+}
+
+int raftcorr_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t dy_batch, int64_t dy_row,
+                            int dtype, int N, int64_t P, int C, int groups, const float* weight, const float* bias, int act,
+                            const float* stats, void* dx, float* dweight, float* dbias,
+                            void* workspace, int64_t workspace_bytes, void* stream)
+{
+    const int rc = check_group_norm("group_norm_bwd", dtype, N, P, C, groups, act, x_row < dy_row ? x_row : dy_row, workspace_bytes, workspace);
+    if (rc) return rc;
+    if (!x || !dy || !stats) return fail(RAFTCORR_EINVAL, "group_norm_bwd: null pointer");
+    return launch_group_norm_bwd(x, x_batch, x_row, dy, dy_batch, dy_row, dtype, N, P, C, groups, weight, bias, act, stats, dx, dweight, dbias,
+                                 workspace, (hipStream_t)stream);
+}
+
+static int check_tensors(const char* who, const void* const* ptrs, const int64_t* numels, int count, int dtype)
+{
+    if (dtype != RAFTCORR_DTYPE_FP32 && dtype != RAFTCORR_DTYPE_BF16) return fail(RAFTCORR_EINVAL, "%s: dtype = %d", who, dtype);
+    if (count < 1 || !ptrs || !numels) return fail(RAFTCORR_EINVAL, "%s: no tensors", who);
+    int64_t tiles = 0;
+    for (int i = 0; i < count; ++i) {
+        if (!ptrs[i]) return fail(RAFTCORR_EINVAL, "%s: tensor %d is null", who, i);
+        if (numels[i] < 1) return fail(RAFTCORR_EINVAL, "%s: tensor %d has %lld values", who, i, (long long)numels[i]);
+        tiles += (numels[i] - 1) / RAFTCORR_ADAMW_TILE + 1;
+        if (tiles > kMostBlocks) return fail(RAFTCORR_EUNSUPPORTED, "%s: more than %lld tiles of %d values", who, (long long)kMostBlocks, RAFTCORR_ADAMW_TILE);
+    }
+    return RAFTCORR_OK;
+}
+
+int64_t raftcorr_adamw_norm_partials(const int64_t* numels, int count)
+{
+    if (!numels || count < 1) return 0;
+    for (int i = 0; i < count; ++i)
+        if (numels[i] < 1) return 0;
+    return adamw_norm_partials(numels, count);
+}
+
+int raftcorr_adamw_norm(const void* const* grads, const int64_t* numels, int count, int dtype, double* partial, void* stream)
+{
+    const int rc = check_tensors("adamw_norm", grads, numels, count, dtype);
+    if (rc) return rc;
+    if (!partial) return fail(RAFTCORR_EINVAL, "adamw_norm: null pointer");
+    return launch_adamw_norm(grads, numels, count, dtype, partial, (hipStream_t)stream);
+}
+
+int raftcorr_adamw_step(void* const* params, const void* const* grads, const int64_t* numels, const int64_t* offsets,
+                        const int32_t* slots, int count, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,
+                        uint8_t* exp_avg_exp, uint8_t* exp_avg_sq_exp, float* steps, float* scale,
+                        double lr, const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                        uint32_t seed, const double* partial, int partials, double max_norm, double* clip, float* norm,
+                        void* stream)
+{
+    int rc = check_tensors("adamw_step", params, numels, count, dtype);
+    if (!rc) rc = check_tensors("adamw_step", grads, numels, count, dtype);
+    if (rc) return rc;
+    if (state_bits != 32 && state_bits != 8) return fail(RAFTCORR_EINVAL, "adamw_step: state_bits = %d", state_bits);
+    if (!offsets || !slots || !exp_avg || !exp_avg_sq || !steps || !scale || (state_bits == 8 && (!exp_avg_exp || !exp_avg_sq_exp)))
+        return fail(RAFTCORR_EINVAL, "adamw_step: null pointer");
+    for (int i = 0; i < count; ++i)
+        if (offsets[i] < 0 || offsets[i] % RAFTCORR_ADAMW_TILE || offsets[i] / RAFTCORR_ADAMW_TILE > 0xFFFFFFFFLL || slots[i] < 0)
+            return fail(RAFTCORR_EINVAL, "adamw_step: tensor %d has offset %lld, slot %d", i, (long long)offsets[i], slots[i]);
+    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 && weight_decay >= 0.0) || (!lr_device && !(lr >= 0.0)))
+        return fail(RAFTCORR_EINVAL, "adamw_step: lr = %g, betas = (%g, %g), eps = %g, weight_decay = %g", lr, beta1, beta2, eps, weight_decay);
+    if (partials < 0 || (partials && (!partial || !clip || !norm || !(max_norm > 0.0))))
+        return fail(RAFTCORR_EINVAL, "adamw_step: %d partial sums, max_norm = %g", partials, max_norm);
+    return launch_adamw_step(params, grads, numels, offsets, slots, count, dtype, state_bits, exp_avg, exp_avg_sq, exp_avg_exp, exp_avg_sq_exp,
+                             steps, scale, lr, lr_device, beta1, beta2, eps, weight_decay, seed, partial, partials, max_norm, clip, norm,
+                             (hipStream_t)stream);
+}
+
+int raftcorr_adamw_decode(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_exp, const uint8_t* exp_avg_sq_exp,
+                          int64_t count, int dtype, void* m, void* v, void* stream)
+{
+    if (dtype != RAFTCORR_DTYPE_FP32 && dtype != RAFTCORR_DTYPE_BF16) return fail(RAFTCORR_EINVAL, "adamw_decode: dtype = %d", dtype);
+    if (!exp_avg || !exp_avg_sq || !exp_avg_exp || !exp_avg_sq_exp || !m || !v) return fail(RAFTCORR_EINVAL, "adamw_decode: null pointer");
+    if (count < 1 || count % RAFTCORR_ADAMW_TILE || count / RAFTCORR_ADAMW_TILE > kMostBlocks)
+        return fail(RAFTCORR_EINVAL, "adamw_decode: %lld values are no whole tiles", (long long)count);
+    return launch_adamw_decode(exp_avg, exp_avg_sq, exp_avg_exp, exp_avg_sq_exp, count, dtype, m, v, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -87,6 +87,21 @@ int launch_alt_lookup_bwd16(const void* f1t, const void* const* f2t, const float
                             void* workspace, size_t workspace_bytes, hipStream_t s, const void* f1p_window = nullptr,
                             const void* groups = nullptr);
 
+size_t group_norm_workspace_bytes(int N, int C, int G);
+int launch_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int G, const float* w,
+                          const float* b, float eps, int act, void* y, float* stats, void* workspace, hipStream_t s);
+int launch_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t d_batch, int64_t d_row, int dtype, int N,
+                          int64_t P, int C, int G, const float* w, const float* b, int act, const float* stats, void* dx, float* dw,
+                          float* db, void* workspace, hipStream_t s);
+int64_t adamw_norm_partials(const int64_t* numels, int count);
+int launch_adamw_norm(const void* const* grads, const int64_t* numels, int count, int dtype, double* partial, hipStream_t s);
+int launch_adamw_step(void* const* params, const void* const* grads, const int64_t* numels, const int64_t* offsets, const int32_t* slots,
+                      int count, int dtype, int bits, void* m, void* v, uint8_t* me, uint8_t* ve, float* steps, float* scale,
+                      double lr, const float* lr_device, double b1, double b2, double eps, double wd, uint32_t seed,
+                      const double* partial, int partials, double max_norm, double* clip, float* norm, hipStream_t s);
+int launch_adamw_decode(const uint8_t* m, const uint8_t* v, const uint8_t* me, const uint8_t* ve, int64_t count, int dtype, void* mo, void* vo,
+                        hipStream_t s);
+
 // floor + fraction of a sampling coordinate, memory-safe for NaN / huge values: anything
 // that is not a sane pixel coordinate is pushed far outside the map (all taps read as zero).
 __device__ __forceinline__ void split_coord(float x, int& x0, float& fx) {
