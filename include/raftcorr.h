@@ -384,22 +384,23 @@ int raftcorr_alt_features_bwd(const float* d1, const float* const* d2_levels, in
  * channels, element (n, p, c) at x[n * x_batch + p * x_row + c]; groups neighbouring channels share mean and (biased) variance:
  *   y = act((x - mean) * rstd * weight[c] + bias[c]),  rstd = 1 / sqrt(var + eps)
  *   weight, bias  (C) float32, each may be NULL (1 and 0).     y: (N, P, C) dense, type of x.
- *   stats         (N, groups, 2) float32: mean and rstd, always written; the backward call reads it.
+ *   stats         (N, groups, 2) float64: mean and rstd, always written; the backward call reads it.
  *   workspace     raftcorr_group_norm_workspace_bytes(N, C, groups) bytes, 16-byte aligned, contents don't-care.
  * Backward: dy as x (strides of its own), dx (N, P, C) dense or NULL, dweight / dbias (C) float32 or NULL, all overwritten.
- * relu'(0) = 0.  Statistics and sums are float32; no atomics, the same bits on every call.  x, dy, y, dx need no more than their
+ * relu'(0) = 0, and ReLU's side is that of z in 64 bits.  Statistics are summed in float64, gradients in float32; no atomics, the same
+ * bits on every call.  x, dy, y, dx need no more than their
  * element's alignment.  Any C, groups that divide it, P, N >= 1; row stride >= C unless P == 1.
- * RAFTCORR_EUNSUPPORTED beyond 2^24 - 1 workgroups (N, N * groups / 4 or C / 4 of that order). */
+ * RAFTCORR_EUNSUPPORTED where N * groups + C passes 2^22 or C passes 2^20. */
 #define RAFTCORR_ACT_NONE 0
 #define RAFTCORR_ACT_RELU 1
 #define RAFTCORR_ACT_SILU 2
 int64_t raftcorr_group_norm_workspace_bytes(int N, int C, int groups);
 int raftcorr_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int groups,
-                            const float* weight, const float* bias, double eps, int act, void* y, float* stats,
+                            const float* weight, const float* bias, double eps, int act, void* y, double* stats,
                             void* workspace, int64_t workspace_bytes, void* stream);
 int raftcorr_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t dy_batch, int64_t dy_row,
                             int dtype, int N, int64_t P, int C, int groups, const float* weight, const float* bias, int act,
-                            const float* stats, void* dx, float* dweight, float* dbias,
+                            const double* stats, void* dx, float* dweight, float* dbias,
                             void* workspace, int64_t workspace_bytes, void* stream);
 
 /* One AdamW step of many tensors (replaces torch.optim.AdamW + clip_grad_norm_ of core/train_origin.py:84-95,210-216):

@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(_HERE, "libraftcorr.so")
 MAX_LEVELS = 8
 PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2, "fp16x2": 3}          # RAFTCORR_PREC_*
 VOLUMES = {"fp32": 0, "fp16": 1, "bf16": 2}                              # RAFTCORR_VOL_*
-DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}     # RAFTCORR_DTYPE_*, by str(tensor.dtype)
+DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}  # RAFTCORR_DTYPE_*, by str(tensor.dtype)
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}                          # RAFTCORR_ACT_*
 ADAMW_TILE, ADAMW_BLOCK = 512, 64                                        # RAFTCORR_ADAMW_*
 MODE_FORK = 0
@@ -131,6 +131,23 @@ def load():
         f"raft_amd: the HIP extension {LIB_PATH} is not available ({_load_error}); build it with "
         "`python -c 'import __graft_entry__ as g; g.build()'` or `make -C raft_amd/csrc`. "
         "There is no CPU fallback.")
+
+
+_glue = None
+
+
+def glue():
+    """The PyTorch glue of the norm and the optimizer (csrc/glue.cpp), or RuntimeError (never falls back)."""
+    global _glue
+    if _glue is None:
+        load()
+        import torch                                    # noqa: F401  (its libraries first)
+        try:
+            from . import _glue as module
+        except ImportError as e:
+            raise RuntimeError(f"raft_amd: the extension raft_amd/_glue.so is not available ({e}); build it with `make -C raft_amd/csrc`")
+        _glue = module
+    return _glue
 
 
 _fast = {}

@@ -1,10 +1,9 @@
 """The optimizer step of RAFT's training recipe -- AdamW behind clip_grad_norm_ (core/train_origin.py:84-95,210-216) -- over all
 tensors of a model in a few launches, with moments in 32 or in 8 bits, backed by libraftcorr.so (C ABI in include/raftcorr.h).
 
-PyTorch is used for device memory, streams and the optimizer's bookkeeping only; there is no fallback path.
+PyTorch is used for device memory, streams and the optimizer's bookkeeping only (csrc/glue.cpp walks the parameters); there is no
+fallback path.
 """
-import ctypes
-
 import torch
 
 from . import _lib
@@ -15,23 +14,6 @@ __all__ = ["AdamW"]
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
-def _dense(p):
-    """Whether the tensor's values fill one stretch of memory without gaps or overlaps, in whatever order."""
-    if p.is_contiguous():
-        return True
-    want = 1
-    for s, n in sorted((s, n) for n, s in zip(p.shape, p.stride()) if n > 1):
-        if s != want:
-            return False
-        want *= n
-    return True
-
-
-def _order(t):
-    """The strides that say where the values lie (those of axes of one value do not)."""
-    return [s for n, s in zip(t.shape, t.stride()) if n > 1]
-
-
 class _Bucket:
     """The parameters of one group that share device and type, and their state in flat buffers: parameter i's moments start at
     value offsets[i], a multiple of the tile, in the order of the parameter's own memory."""
@@ -39,19 +21,14 @@ class _Bucket:
     def __init__(self, params, bits, index):
         self.params, self.bits, self.index = params, bits, index
         self.device, self.dtype = params[0].device, params[0].dtype
-        self.numels = [p.numel() for p in params]
-        self.strides = [p.stride() for p in params]
-        self.offsets, total = [], 0
-        for n in self.numels:
-            self.offsets.append(total)
-            total += (n + _lib.ADAMW_TILE - 1) // _lib.ADAMW_TILE * _lib.ADAMW_TILE
-        self.total = total
+        self.glue = _lib.glue().Bucket(params)
+        self.numels, self.offsets, self.total = self.glue.numels, self.glue.offsets, self.glue.total
+        total = self.total
         kind = torch.float32 if bits == 32 else torch.uint8
         self.m, self.v = (torch.zeros(total, dtype=kind, device=self.device) for _ in range(2))
         blocks = 0 if bits == 32 else total // _lib.ADAMW_BLOCK
         self.me, self.ve = (torch.zeros(blocks, dtype=torch.uint8, device=self.device) for _ in range(2))
         self.steps = torch.zeros(len(params), dtype=torch.float32, device=self.device)
-        self.host = {}                                       # host arrays of a set of present gradients
 
     def views(self, i):
         """The state of parameter i as it stands in the optimizer's state."""
@@ -63,17 +40,6 @@ class _Bucket:
             first, last = at // _lib.ADAMW_BLOCK, (at + self.numels[i] + _lib.ADAMW_BLOCK - 1) // _lib.ADAMW_BLOCK
             out["exp_avg_exponent"], out["exp_avg_sq_exponent"] = self.me[first:last], self.ve[first:last]
         return out
-
-    def arrays(self, present):
-        """numels, offsets, slots of the parameters `present` (a tuple of indices) as host arrays."""
-        got = self.host.get(present)
-        if got is None:
-            if len(self.host) > 8:
-                self.host.clear()
-            n = len(present)
-            got = self.host[present] = ((ctypes.c_int64 * n)(*[self.numels[i] for i in present]),
-                                        (ctypes.c_int64 * n)(*[self.offsets[i] for i in present]), (ctypes.c_int32 * n)(*present))
-        return got
 
 
 class AdamW(torch.optim.Optimizer):
@@ -87,8 +53,9 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters: CUDA, float32 or bfloat16 (rounded stochastically; no 32-bit copy is kept), in one stretch of memory.
     Gradients: of the parameters' type; parameters without one are passed over.  A step can be captured into a HIP graph once
-    one step has been taken; numbers among its options stay what they were.  `state` holds views ("step", "exp_avg", "exp_avg_sq", with 8 bits their codes and exponents) into
-    one buffer a bucket of parameters (write into them; another tensor put in their place is not seen); torch.optim.AdamW's state_dict can be loaded with state_bits=32 and the other way round.
+    one step has been taken; numbers among its options stay what they were.  `state` holds views ("step", "exp_avg", "exp_avg_sq",
+    with 8 bits their codes and exponents) into one buffer a bucket of parameters: write into them, another tensor put in their
+    place is not seen.  torch.optim.AdamW's state_dict can be loaded with state_bits=32, and the other way round.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None, seed=0):
@@ -136,8 +103,6 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("parameter must be a CUDA tensor")
                 if p.dtype not in _DTYPES:
                     raise RuntimeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
-                if not _dense(p):
-                    raise RuntimeError(f"parameter of shape {tuple(p.shape)} and strides {p.stride()} does not lie in one stretch of memory")
                 if p.numel():
                     by_kind.setdefault((p.device, p.dtype), []).append(p)
             made.append([])
@@ -208,42 +173,27 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = [(group, b) + _gather(b) for group, buckets in zip(self.param_groups, self._ready()) for b in buckets]
-        work = [w for w in work if w[2]]
-        max_norm = self.defaults["max_norm"]
-        if not work:
-            self.grad_norm = None if max_norm is None else torch.zeros(())
-            return loss
-        lib = _lib.load()
-        partial, partials, pieces = None, 0, []
+        buckets = self._ready()
+        work = [(group, b) for group, of in zip(self.param_groups, buckets) for b in of if b.glue.collect(b.params)]
+        max_norm, partial, self.grad_norm = self.defaults["max_norm"], None, None
         if max_norm is not None:
-            if len({b.device for _, b, *_ in work}) > 1:
+            device = work[0][1].device if work else None
+            if any(b.device != device for _, b in work):
                 raise RuntimeError("max_norm: the parameters are on more than one device")
-            pieces = [lib.raftcorr_adamw_norm_partials(arrays[0], len(present)) for _, _, present, arrays, *_ in work]
-            partials = sum(pieces)
-            first = work[0][1]
-            partial = torch.empty(partials + 1, dtype=torch.float64, device=first.device)      # the last one: the coefficient
-            self.grad_norm = torch.empty((), dtype=torch.float32, device=first.device)
-            at = partial.data_ptr()
-            for (_, b, present, arrays, _, grads, _), n in zip(work, pieces):
-                with _guard(partial):
-                    _lib.check(lib.raftcorr_adamw_norm(grads, arrays[0], len(present), _lib.DTYPES[str(b.dtype)], at, _stream(partial)),
-                               "adamw_norm")
-                at += 8 * n
-        for group, b, present, (numels, offsets, slots), params, grads, keep in work:
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=device) if work else torch.zeros(())
+            if work:
+                pieces = [b.glue.partials() for _, b in work]
+                partial, at = torch.empty(sum(pieces) + 1, dtype=torch.float64, device=device), 0      # the last one: the coefficient
+                for (_, b), n in zip(work, pieces):
+                    b.glue.norm(partial, at)
+                    at += n
+        for group, b in work:
             lr, (b1, b2) = group["lr"], group["betas"]
-            on_device = torch.is_tensor(lr) and lr.is_cuda
-            if on_device and lr.device != b.device:
+            on_device = lr if torch.is_tensor(lr) and lr.is_cuda else None
+            if on_device is not None and on_device.device != b.device:
                 raise RuntimeError(f"lr is on {lr.device}, expected {b.device}")
-            scale = torch.empty(2 * len(b.params), dtype=torch.float32, device=b.device)
-            with _guard(scale):
-                _lib.check(lib.raftcorr_adamw_step(
-                    params, grads, numels, offsets, slots, len(present), _lib.DTYPES[str(b.dtype)], b.bits, b.m.data_ptr(), b.v.data_ptr(),
-                    b.me.data_ptr() if b.bits == 8 else None, b.ve.data_ptr() if b.bits == 8 else None, b.steps.data_ptr(), scale.data_ptr(),
-                    0.0 if on_device else float(lr), lr.data_ptr() if on_device else None, b1, b2, group["eps"], group["weight_decay"],
-                    (group["seed"] + 7919 * b.index) & 0xFFFFFFFF, partial.data_ptr() if partials else None, partials, max_norm or 0.0,
-                    partial.data_ptr() + 8 * partials if partials else None, self.grad_norm.data_ptr() if partials else None,
-                    _stream(scale)), "adamw_step")
+            b.glue.step(b.bits, b.m, b.v, b.me, b.ve, b.steps, on_device, 0.0 if on_device is not None else float(lr), b1, b2, group["eps"],
+                        group["weight_decay"], (group["seed"] + 7919 * b.index) & 0xFFFFFFFF, partial, max_norm or 0.0, self.grad_norm)
         return loss
 
 
@@ -271,32 +221,7 @@ def _adopt(views, old, bits):
     for name in names:
         if old[name].shape != views[name].shape:
             raise RuntimeError(f"the loaded {name} has shape {tuple(old[name].shape)}, expected {tuple(views[name].shape)}")
-        if bits == 8 and _order(old[name]) != _order(views[name]):
+        if bits == 8 and not _lib.glue().same_order(old[name], views[name]):
             raise RuntimeError(f"the loaded {name} has another memory order than the parameter: its blocks of 8-bit values differ")
         views[name].copy_(old[name])
     views["step"].fill_(float(old["step"]))
-
-
-def _gather(b):
-    """(indices of the parameters with a gradient, their host arrays, parameter and gradient addresses, what must stay alive)."""
-    present, ps, gs, keep = [], [], [], []
-    for i, p in enumerate(b.params):
-        g = p.grad
-        if g is None:
-            continue
-        if g.dtype != b.dtype or g.device != b.device or g.layout != torch.strided:
-            raise RuntimeError(f"gradient is {g.dtype}, {g.layout} on {g.device}, expected a dense {b.dtype} on {b.device}")
-        if p.dtype != b.dtype or p.device != b.device or p.numel() != b.numels[i]:
-            raise RuntimeError("a parameter's type, device or size has changed since the state was made")
-        strides = p.stride()
-        if strides != b.strides[i] and [s for n, s in zip(p.shape, b.strides[i]) if n > 1] != _order(p):
-            raise RuntimeError("a parameter's memory order has changed since the state was made")
-        if g.stride() != strides and _order(g) != _order(p):
-            g = torch.empty_like(p).copy_(g)                     # the order of the parameter's memory
-            keep.append(g)
-        present.append(i)
-        ps.append(p.data_ptr())
-        gs.append(g.data_ptr())
-    n = len(ps)
-    present = tuple(present)
-    return present, b.arrays(present) if n else None, (ctypes.c_void_p * n)(*ps), (ctypes.c_void_p * n)(*gs), keep

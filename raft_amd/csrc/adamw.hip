@@ -3,9 +3,9 @@
 //   c = min(1, max_norm / (|g| + 1e-6)),  m = b1 m + (1 - b1) c g,  v = b2 v + (1 - b2) (c g)^2,
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// Memory bound: 28 bytes a float32 parameter with 32-bit moments, 16 with 8-bit ones, some 20 operations.  Launches: sums of
-// squares of the gradients (only with clipping), one workgroup that counts the steps and joins the sums, the update; each takes
-// the tensors' addresses by value, as many as 4 KB of kernel arguments hold, so a captured graph depends on no table.
+// Memory bound: 28 bytes a float32 parameter with 32-bit moments, 16 with 8-bit ones.  Launches: sums of squares of the gradients
+// (only with clipping), one workgroup that counts the steps and joins the sums, the update; each takes the tensors' addresses by
+// value, as many as 4 KB of kernel arguments hold, so a captured graph depends on no table.
 //
 // The moments of a bucket of tensors lie in flat buffers; tensor i starts at a multiple of 512 values.  A wave takes 512
 // neighbouring values ("tile") of one tensor, 8 a lane.
@@ -18,6 +18,10 @@
 // value come from (seed, step, position) alone.  A second moment that is not zero keeps at least one unit: m / (sqrt(0) + eps)
 // would be a huge step.  E = 255 (something not finite in the block) decodes as NaN, all 64; E = 0 (all below 2^-126) as zero.
 // The new moments are summed in 64 bits (full rate here), rounded to 32, used for the update, then coded.
+//
+// A code is the upper bits of a float32 whose unit is 2^-129: subnormal below 8 units, three mantissa bits above.  So the float with
+// the bits c << 20, times a power of two, is the value; and the other way round the value times that power, its bits, the random
+// bits added below the code's last one, shifted down by 20, is the code.  No case apart for small codes.
 #include "common.h"
 #include "elem.h"
 
@@ -28,14 +32,14 @@ static_assert(kTile == 64 * kLane && kBlock % kLane == 0 && kTile % kBlock == 0,
 
 // ---- gradient norm ------------------------------------------------------------------------------------------------------
 
-enum { kNormTensors = 240 };
+enum { kNormTensors = 240, kRun = 4 };
 struct NormTable {
     const void* grad[kNormTensors];
     uint32_t first[kNormTensors];             // first tile of each tensor, counted from the first tensor of the launch
     uint16_t tail[kNormTensors];              // values in its last tile
 };
 
-// the tensor a tile belongs to: the last one that starts at or before it
+// the tensor a tile belongs to: the last of `count` that starts at or before it
 __device__ __forceinline__ int tensor_of(const uint32_t* first, int count, uint32_t tile)
 {
     int lo = 0, hi = count;
@@ -53,25 +57,48 @@ __device__ __forceinline__ double wave_sum(double v)
     return v;
 }
 
-// partial[block] = sum of squares over the tiles of the block's waves, in 64 bits
+// partial[block] = sum of squares over the tiles of the block's waves, in 64 bits.  A wave takes `run` neighbouring tiles: it looks
+// its tensor up once and has the loads of four tiles on their way at a time.
 template <typename T>
-__global__ __launch_bounds__(kWg) void adamw_norm_kernel(NormTable tab, int count, uint32_t tiles, double* __restrict__ partial)
+__global__ __launch_bounds__(kWg) void adamw_norm_kernel(NormTable tab, int count, uint32_t tiles, uint32_t run, double* __restrict__ partial)
 {
     __shared__ double part[kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63;
     double sum = 0.0;
-    for (uint32_t tile = blockIdx.x * kWaves + wave; tile < tiles; tile += gridDim.x * kWaves) {
-        const int i = tensor_of(tab.first, count, tile);
-        const uint32_t next = i + 1 < count ? tab.first[i + 1] : tiles;
-        const int values = tile + 1 == next ? tab.tail[i] : kTile;
-        const T* g = (const T*)tab.grad[i] + (int64_t)(tile - tab.first[i]) * kTile + lane * kLane;
-        const int have = values - lane * kLane;
-        if (have >= kLane) {
-            const Vec<T, kLane> v = load_vec<T, kLane>(g);
+    uint32_t tile = (blockIdx.x * kWaves + wave) * run;
+    const uint32_t end = min(tile + run, tiles);
+    if (tile < end) {
+        int i = tensor_of(tab.first, count, tile);
+        while (tile < end) {
+            const uint32_t first = tab.first[i], next = i + 1 < count ? tab.first[i + 1] : tiles;
+            const T* g = (const T*)tab.grad[i] + (int64_t)(tile - first) * kTile + lane * kLane;
+            const uint32_t full = min(end, next - 1);          // whole tiles up to here
+            for (; tile + kRun <= full; tile += kRun, g += kRun * kTile) {
+                Vec<T, kLane> v[kRun];
 #pragma unroll
-            for (int j = 0; j < kLane; ++j) { const double e = (double)to_float(v[j]); sum += e * e; }
-        } else {
-            for (int j = 0; j < have; ++j) { const double e = (double)to_float(g[j]); sum += e * e; }
+                for (int u = 0; u < kRun; ++u) v[u] = load_vec<T, kLane>(g + u * kTile);
+#pragma unroll
+                for (int u = 0; u < kRun; ++u)
+#pragma unroll
+                    for (int j = 0; j < kLane; ++j) { const double e = (double)to_float(v[u][j]); sum += e * e; }
+            }
+            for (; tile < full; ++tile, g += kTile) {
+                const Vec<T, kLane> v = load_vec<T, kLane>(g);
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) { const double e = (double)to_float(v[j]); sum += e * e; }
+            }
+            if (tile < end) {                                   // the tensor's last tile
+                const int have = (int)tab.tail[i] - lane * kLane;
+                if (have >= kLane) {
+                    const Vec<T, kLane> v = load_vec<T, kLane>(g);
+#pragma unroll
+                    for (int j = 0; j < kLane; ++j) { const double e = (double)to_float(v[j]); sum += e * e; }
+                } else {
+                    for (int j = 0; j < have; ++j) { const double e = (double)to_float(g[j]); sum += e * e; }
+                }
+                ++tile;
+                ++i;
+            }
         }
     }
     sum = wave_sum(sum);
@@ -89,28 +116,40 @@ __global__ __launch_bounds__(kWg) void adamw_norm_kernel(NormTable tab, int coun
 enum { kStepTensors = 960 };
 struct StepTable { int32_t slot[kStepTensors]; };
 
-// counts the tensors' steps; scale[slot] = (lr / (1 - b1^t), 1 / sqrt(1 - b2^t)); joins the partial sums (partials > 0)
-__global__ __launch_bounds__(kWg) void adamw_count_kernel(StepTable tab, int count, float* __restrict__ steps, float2* __restrict__ scale,
-                                                          double lr, const float* __restrict__ lr_device, double b1, double b2,
-                                                          const double* __restrict__ partial, int partials, double max_norm,
-                                                          double* __restrict__ clip, float* __restrict__ norm)
+enum { kCountWg = 1024 };
+
+// b^t for a whole t
+__device__ __forceinline__ double power(double b, uint32_t t)
 {
+    double p = 1.0;
+    for (; t; t >>= 1, b *= b)
+        if (t & 1) p *= b;
+    return p;
+}
+
+// counts the tensors' steps; scale[slot] = (lr / (1 - b1^t), 1 / sqrt(1 - b2^t)); joins the partial sums (partials > 0)
+__global__ __launch_bounds__(kCountWg) void adamw_count_kernel(StepTable tab, int count, float* __restrict__ steps, float2* __restrict__ scale,
+                                                               double lr, const float* __restrict__ lr_device, double b1, double b2,
+                                                               const double* __restrict__ partial, int partials, double max_norm,
+                                                               double* __restrict__ clip, float* __restrict__ norm)
+{
+    __shared__ double part[kCountWg / 64];
+    double sum = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < partials; i += kCountWg) sum += partial[i];
     if (lr_device) lr = (double)*lr_device;
-    for (int i = threadIdx.x; i < count; i += kWg) {
-        const int slot = tab.slot[i];
+    if ((int)threadIdx.x < count) {
+        const int slot = tab.slot[threadIdx.x];
         const float t = steps[slot] + 1.f;
         steps[slot] = t;
-        scale[slot] = make_float2((float)(lr / (1.0 - pow(b1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)t))));
+        scale[slot] = make_float2((float)(lr / (1.0 - power(b1, (uint32_t)t))), (float)(1.0 / sqrt(1.0 - power(b2, (uint32_t)t))));
     }
     if (!partials) return;
-    __shared__ double part[kWaves];
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < partials; i += kWg) sum += partial[i];
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = sum;
     __syncthreads();
     if (threadIdx.x) return;
-    for (int w = 1; w < kWaves; ++w) sum += part[w];
+    for (int w = 1; w < kCountWg / 64; ++w) sum += part[w];
     sum = sqrt(sum);
     const double c = max_norm / (sum + 1e-6);
     *clip = c > 1.0 ? 1.0 : c;                  // (a NaN stays one)
@@ -119,14 +158,12 @@ __global__ __launch_bounds__(kWg) void adamw_count_kernel(StepTable tab, int cou
 
 // ---- update -------------------------------------------------------------------------------------------------------------
 
-enum { kStepWords = 32, kUpdateTensors = 120 };
-struct UpdateTensor {
-    void* p;
-    const void* g;
-    uint32_t first, state;                      // first tile in the launch, first tile in the bucket's buffers
-    uint32_t slot, tail;
+enum { kUpdateTensors = 140 };
+struct UpdateTable {
+    uint64_t p[kUpdateTensors], g[kUpdateTensors];
+    uint32_t first[kUpdateTensors], state[kUpdateTensors];      // first tile in the launch, first tile in the bucket's buffers
+    uint32_t slot_tail[kUpdateTensors];                         // step counter << 10 | values in the last tile
 };
-struct UpdateTable { UpdateTensor t[kUpdateTensors]; };
 
 struct UpdateArgs {
     void* m;
@@ -154,37 +191,48 @@ __device__ __forceinline__ uint32_t mix(uint32_t x)
 }
 constexpr uint32_t kGolden = 0x9E3779B9u;       // leading binary digits of the golden ratio: neighbouring positions land far apart
 
-// the largest of 8 lanes' values (the lanes of one block)
-__device__ __forceinline__ float block_max(float v)
+// the largest of the values of a block's lanes
+__device__ __forceinline__ uint32_t block_max(uint32_t v)
 {
 #pragma unroll
-    for (int o = 1; o < kBlock / kLane; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+    for (int o = 1; o < kBlock / kLane; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
     return v;
 }
 
-// |x| of exponent at most E, in units of 2^(E - 127 - top), to its code: below 8 units 8 is added, which lines the units up with the
-// same bit of the word that ends the three mantissa bits above; the random bits then carry into it or not.
-__device__ __forceinline__ uint32_t encode(float x, int shift, uint32_t bits16)
-{
-    const float u = ldexpf(x, shift);
-    const bool low = u < 8.f;
-    const uint32_t w = __float_as_uint(low ? u + 8.f : u) + (bits16 << 4);
-    return (w >> 20) - ((0x41000000u >> 20) - (low ? 0u : 8u));
-}
-
-__device__ __forceinline__ double decode(uint32_t code, int shift)
-{
-    const uint32_t units = code < 8 ? code : 8 + (code & 7);
-    return ldexp((double)units, shift + (code < 8 ? 0 : (int)(code >> 3) - 1));
-}
+// 2^e for -1022 <= e <= 1023
+__device__ __forceinline__ double exp2i(int e) { return __longlong_as_double((long long)(e + 1023) << 52); }
 
 template <typename T> __device__ __forceinline__ T round_param(float x, uint32_t) { return (T)x; }
 // bfloat16 parameters are rounded up with the probability of what is dropped: a step of 2^-9 of a weight would be lost otherwise
+// (infinities and NaN as they are: x comes out of a sum, its NaN have their upper mantissa bit set)
 template <> __device__ __forceinline__ __bf16 round_param<__bf16>(float x, uint32_t bits16)
 {
     const uint32_t w = __float_as_uint(x);
-    if ((w & 0x7F800000u) == 0x7F800000u) return (__bf16)x;                   // infinities and NaN as they are
-    return __builtin_bit_cast(__bf16, (uint16_t)((w + bits16) >> 16));
+    return __builtin_bit_cast(__bf16, (uint16_t)((w + (__builtin_isfinite(x) ? bits16 : 0u)) >> 16));
+}
+
+// m / (sqrt(v) r + eps) within four units of 2^-24.  The root instruction takes subnormals for zero: with eps >= 1e-12 that is below
+// the rounding of the sum (EXACT = false), else they are scaled.
+template <bool EXACT> __device__ __forceinline__ float quotient(float m, float v, float r, float eps)
+{
+    float s;
+    if (EXACT) {
+        const bool low = v < 0x1p-96f;
+        s = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v) * (low ? 0x1p-32f : 1.f);
+    } else {
+        s = __builtin_amdgcn_sqrtf(v);
+    }
+    return m * __builtin_amdgcn_rcpf(s * r + eps);
+}
+
+// byte j of w as a code of the first / second moment: the float whose bits are the code << 20 (and the sign)
+__device__ __forceinline__ float code_float_signed(uint32_t w, int j) { return __uint_as_float((uint32_t)((int32_t)(w << (24 - 8 * j)) >> 4) & 0x87F00000u); }
+__device__ __forceinline__ float code_float(uint32_t w, int j) { return __uint_as_float((j < 3 ? w << (20 - 8 * j) : w >> 4) & 0x0FF00000u); }
+
+// the upper bytes of four words as one word
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x07030C0Cu), __builtin_amdgcn_perm(b, a, 0x0C0C0703u), 0x07060100u);
 }
 
 template <typename T, int BITS>
@@ -193,17 +241,13 @@ __global__ __launch_bounds__(kWg) void adamw_update_kernel(UpdateTable tab, Upda
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63;
     const uint32_t tile = blockIdx.x * kWaves + wave;
     if (tile >= a.tiles) return;
-    int lo = 0, hi = (int)a.count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (tab.t[mid].first <= tile) lo = mid; else hi = mid;
-    }
-    const uint32_t first = tab.t[lo].first, next = lo + 1 < (int)a.count ? tab.t[lo + 1].first : a.tiles;
-    const uint32_t slot = tab.t[lo].slot;
-    const int have = min(kLane, (tile + 1 == next ? (int)tab.t[lo].tail : kTile) - lane * kLane);      // may be <= 0
-    T* p = (T*)tab.t[lo].p + (int64_t)(tile - first) * kTile + lane * kLane;
-    const T* g = (const T*)tab.t[lo].g + (int64_t)(tile - first) * kTile + lane * kLane;
-    const int64_t pos = ((int64_t)tab.t[lo].state + (tile - first)) * kTile + lane * kLane;
+    const int lo = tensor_of(tab.first, (int)a.count, tile);
+    const uint32_t first = tab.first[lo], next = lo + 1 < (int)a.count ? tab.first[lo + 1] : a.tiles;
+    const uint32_t slot = tab.slot_tail[lo] >> 10;
+    const int have = min(kLane, (tile + 1 == next ? (int)(tab.slot_tail[lo] & 1023) : kTile) - lane * kLane);      // may be <= 0
+    T* p = (T*)tab.p[lo] + (int64_t)(tile - first) * kTile + lane * kLane;
+    const T* g = (const T*)tab.g[lo] + (int64_t)(tile - first) * kTile + lane * kLane;
+    const int64_t pos = ((int64_t)tab.state[lo] + (tile - first)) * kTile + lane * kLane;
     Vec<T, kLane> pv, gv;
     if (have == kLane) {
         pv = load_vec<T, kLane>(p);
@@ -218,9 +262,9 @@ __global__ __launch_bounds__(kWg) void adamw_update_kernel(UpdateTable tab, Upda
     uint32_t bits[kLane];
     if (BITS == 8 || sizeof(T) == 2) {
         const uint32_t t = (uint32_t)a.steps[slot];
-        const uint32_t key = mix(mix(a.seed + kGolden * t) + (uint32_t)(pos >> 32));
+        const uint32_t key = mix(mix(a.seed + kGolden * t) + (uint32_t)(pos >> 32)) + (uint32_t)pos * kGolden;
 #pragma unroll
-        for (int j = 0; j < kLane; ++j) bits[j] = mix(((uint32_t)pos + j) * kGolden + key);
+        for (int j = 0; j < kLane; ++j) bits[j] = mix(key + j * kGolden);
     }
     float mf[kLane], vf[kLane];
     if (BITS == 32) {
@@ -236,51 +280,58 @@ __global__ __launch_bounds__(kWg) void adamw_update_kernel(UpdateTable tab, Upda
             mv[j] = mf[j];
             vv[j] = vf[j];
         }
-        store_vec<float, kLane>(ms, mv);                       // a tile's state is the bucket's own: whole, padding included
+        store_vec<float, kLane>(ms, mv);                     // a tile's state is the bucket's own: whole, padding included
         store_vec<float, kLane>(vs, vv);
     } else {
         uint8_t* ms = (uint8_t*)a.m + pos;
         uint8_t* vs = (uint8_t*)a.v + pos;
-        Vec<uint8_t, kLane> mv = load_vec<uint8_t, kLane>(ms), vv = load_vec<uint8_t, kLane>(vs);
+        const Vec<uint32_t, 2> mw = load_vec<uint32_t, 2>((const uint32_t*)ms), vw = load_vec<uint32_t, 2>((const uint32_t*)vs);
         const int me = a.me[pos / kBlock], ve = a.ve[pos / kBlock];
-        const double bad = __builtin_nan(""), c1 = 1.0 - a.b1, c2 = 1.0 - a.b2;
-        float mx = 0.f, vx = 0.f;
-        bool finite = true;
+        // value of the float with bits c << 20: unit 2^-129; b1 and b2 go into the factor (an exact product)
+        const double bad = __builtin_nan("");
+        const double mscale = me == 255 ? bad : me == 0 ? 0.0 : a.b1 * exp2i(me - 127 - 16 + 129);
+        const double vscale = ve == 255 ? bad : ve == 0 ? 0.0 : a.b2 * exp2i(ve - 127 - 32 + 129);
+        const double c1 = (1.0 - a.b1) * clip, c2 = (1.0 - a.b2) * clip * clip;
+        uint32_t mx = 0, vx = 0;
 #pragma unroll
         for (int j = 0; j < kLane; ++j) {
-            double m = me == 255 ? bad : me == 0 ? 0.0 : decode(mv[j] & 127, me - 127 - 16);
-            if (mv[j] & 128) m = -m;
-            const double v = ve == 255 ? bad : ve == 0 ? 0.0 : decode(vv[j], ve - 127 - 32);
-            const double e = (double)to_float(gv[j]) * clip;
-            mf[j] = (float)(a.b1 * m + c1 * e);
-            vf[j] = (float)(a.b2 * v + c2 * e * e);
-            mx = fmaxf(mx, fabsf(mf[j]));
-            vx = fmaxf(vx, vf[j]);
-            finite = finite && mf[j] - mf[j] == 0.f && vf[j] - vf[j] == 0.f;
+            const double e = (double)to_float(gv[j]);
+            mf[j] = (float)(c1 * e + mscale * (double)code_float_signed(mw[j / 4], j % 4));
+            vf[j] = (float)(c2 * e * e + vscale * (double)code_float(vw[j / 4], j % 4));
+            mx = max(mx, __float_as_uint(mf[j]) & 0x7FFFFFFFu);         // as whole numbers: NaN and infinity are the largest
+            vx = max(vx, __float_as_uint(vf[j]) & 0x7FFFFFFFu);
         }
-        mx = block_max(finite ? mx : __builtin_inff());
-        vx = block_max(finite ? vx : __builtin_inff());
-        const int mn = (int)(__float_as_uint(mx) >> 23), vn = (int)(__float_as_uint(vx) >> 23);
+        const int mn = (int)(block_max(mx) >> 23), vn = (int)(block_max(vx) >> 23);
+        const uint32_t mlive = mn != 0 && mn != 255 ? ~0u : 0u, vlive = vn != 0 && vn != 255 ? ~0u : 0u;
+        Vec<uint32_t, 2> mo, vo;
 #pragma unroll
-        for (int j = 0; j < kLane; ++j) {
-            uint32_t m = 0, v = 0;
-            if (mn != 0 && mn != 255) m = encode(fabsf(mf[j]), 127 + 16 - mn, bits[j] & 0xFFFF) | (mf[j] < 0.f ? 128u : 0u);
-            if (vn != 0 && vn != 255) {
-                v = encode(vf[j], 127 + 32 - vn, bits[j] >> 16);
-                if (v == 0 && vf[j] > 0.f) v = 1;
+        for (int w = 0; w < 2; ++w) {
+            uint32_t mc[4], vc[4];                              // the code in the upper byte
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = 4 * w + i;
+                const uint32_t mb = __float_as_uint(ldexpf(mf[j], 127 + 16 - 129 - mn)) + ((bits[j] & 0xFFFF) << 4);
+                const uint32_t vb = __float_as_uint(ldexpf(vf[j], 127 + 32 - 129 - vn)) + (bits[j] >> 16 << 4);
+                mc[i] = (mb & 0x80000000u) | (mb << 4 & 0x7FFFFFFFu);
+                vc[i] = max(vb, min(__float_as_uint(vf[j]), 1u) << 20) << 4;
             }
-            mv[j] = (uint8_t)m;
-            vv[j] = (uint8_t)v;
+            mo[w] = upper_bytes(mc[0], mc[1], mc[2], mc[3]) & mlive;
+            vo[w] = upper_bytes(vc[0], vc[1], vc[2], vc[3]) & vlive;
         }
-        store_vec<uint8_t, kLane>(ms, mv);
-        store_vec<uint8_t, kLane>(vs, vv);
+        store_vec<uint32_t, 2>((uint32_t*)ms, mo);
+        store_vec<uint32_t, 2>((uint32_t*)vs, vo);
         if (lane % (kBlock / kLane) == 0) { a.me[pos / kBlock] = (uint8_t)mn; a.ve[pos / kBlock] = (uint8_t)vn; }
     }
+    float q[kLane];
+    if (a.eps >= 1e-12f) {
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-        const float n = to_float(pv[j]) * keep - sc.x * mf[j] / (sqrtf(vf[j]) * sc.y + a.eps);
-        pv[j] = round_param<T>(n, sizeof(T) == 2 ? mix(bits[j] + kGolden) & 0xFFFF : 0);
+        for (int j = 0; j < kLane; ++j) q[j] = quotient<false>(mf[j], vf[j], sc.y, a.eps);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) q[j] = quotient<true>(mf[j], vf[j], sc.y, a.eps);
     }
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) pv[j] = round_param<T>(to_float(pv[j]) * keep - sc.x * q[j], sizeof(T) == 2 ? mix(bits[j] + kGolden) & 0xFFFF : 0);
     if (have == kLane) store_vec<T, kLane>(p, pv);
     else
         for (int j = 0; j < kLane; ++j) if (j < have) p[j] = pv[j];
@@ -295,26 +346,31 @@ __global__ __launch_bounds__(kWg) void adamw_decode_kernel(const uint8_t* __rest
 {
     const int64_t pos = ((int64_t)blockIdx.x * kWg + threadIdx.x) * kLane;
     if (pos >= count) return;
-    const Vec<uint8_t, kLane> mc = load_vec<uint8_t, kLane>(m + pos), vc = load_vec<uint8_t, kLane>(v + pos);
+    const Vec<uint32_t, 2> mw = load_vec<uint32_t, 2>((const uint32_t*)(m + pos)), vw = load_vec<uint32_t, 2>((const uint32_t*)(v + pos));
     const int em = me[pos / kBlock], ev = ve[pos / kBlock];
+    const double bad = __builtin_nan("");
+    const double mscale = em == 255 ? bad : em == 0 ? 0.0 : exp2i(em - 127 - 16 + 129), vscale = ev == 255 ? bad : ev == 0 ? 0.0 : exp2i(ev - 127 - 32 + 129);
     Vec<T, kLane> a, b;
 #pragma unroll
     for (int j = 0; j < kLane; ++j) {
-        float x = em == 255 ? __builtin_nanf("") : em == 0 ? 0.f : (float)decode(mc[j] & 127, em - 127 - 16);
-        if (mc[j] & 128) x = -x;
-        a[j] = from_float<T>(x);
-        b[j] = from_float<T>(ev == 255 ? __builtin_nanf("") : ev == 0 ? 0.f : (float)decode(vc[j], ev - 127 - 32));
+        a[j] = from_float<T>((float)(mscale * (double)code_float_signed(mw[j / 4], j % 4)));
+        b[j] = from_float<T>((float)(vscale * (double)code_float(vw[j / 4], j % 4)));
     }
-    store_vec<T, kLane>(mo + pos, a);
-    store_vec<T, kLane>(vo + pos, b);
+    store_vec_once<T, kLane>(mo + pos, a);
+    store_vec_once<T, kLane>(vo + pos, b);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
 static int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
-// workgroups of the norm pass over `tiles` tiles
-static int64_t norm_blocks(int64_t tiles) { const int64_t b = (tiles + kWaves - 1) / kWaves; return b < 1024 ? b : 1024; }
+// neighbouring tiles a wave of the norm pass takes: some 2048 workgroups, whole rounds of loads
+static uint32_t norm_run(int64_t tiles)
+{
+    const int64_t run = tiles / (2048 * kWaves);
+    return run < 1 ? 1 : (uint32_t)((run + kRun - 1) / kRun * kRun);
+}
+static int64_t norm_blocks(int64_t tiles) { const int64_t waves = (tiles + norm_run(tiles) - 1) / norm_run(tiles); return (waves + kWaves - 1) / kWaves; }
 
 int64_t adamw_norm_partials(const int64_t* numels, int count)
 {
@@ -343,8 +399,8 @@ int launch_adamw_norm(const void* const* grads, const int64_t* numels, int count
             tiles += (uint32_t)t;
         }
         const unsigned blocks = (unsigned)norm_blocks(tiles);
-        if (dtype == RAFTCORR_DTYPE_FP32) adamw_norm_kernel<float><<<blocks, kWg, 0, s>>>(tab, n, tiles, partial);
-        else adamw_norm_kernel<__bf16><<<blocks, kWg, 0, s>>>(tab, n, tiles, partial);
+        if (dtype == RAFTCORR_DTYPE_FP32) adamw_norm_kernel<float><<<blocks, kWg, 0, s>>>(tab, n, tiles, norm_run(tiles), partial);
+        else adamw_norm_kernel<__bf16><<<blocks, kWg, 0, s>>>(tab, n, tiles, norm_run(tiles), partial);
         partial += blocks;
         i += n;
     }
@@ -360,7 +416,7 @@ int launch_adamw_step(void* const* params, const void* const* grads, const int64
         StepTable tab;
         const int n = count - i < kStepTensors ? count - i : kStepTensors;
         for (int k = 0; k < n; ++k) tab.slot[k] = slots[i + k];
-        adamw_count_kernel<<<1, kWg, 0, s>>>(tab, n, steps, (float2*)scale, lr, lr_device, b1, b2, partial, i == 0 ? partials : 0,
+        adamw_count_kernel<<<1, kCountWg, 0, s>>>(tab, n, steps, (float2*)scale, lr, lr_device, b1, b2, partial, i == 0 ? partials : 0,
                                              max_norm, clip, norm);
     }
     for (int i = 0; i < count;) {
@@ -369,8 +425,11 @@ int launch_adamw_step(void* const* params, const void* const* grads, const int64
         const int n = count - i < kUpdateTensors ? count - i : kUpdateTensors;
         for (int k = 0; k < n; ++k) {
             const int64_t t = tiles_of(numels[i + k]);
-            tab.t[k] = UpdateTensor{params[i + k], grads[i + k], tiles, (uint32_t)(offsets[i + k] / kTile), (uint32_t)slots[i + k],
-                                    (uint32_t)(numels[i + k] - (t - 1) * kTile)};
+            tab.p[k] = (uint64_t)params[i + k];
+            tab.g[k] = (uint64_t)grads[i + k];
+            tab.first[k] = tiles;
+            tab.state[k] = (uint32_t)(offsets[i + k] / kTile);
+            tab.slot_tail[k] = (uint32_t)slots[i + k] << 10 | (uint32_t)(numels[i + k] - (t - 1) * kTile);
             tiles += (uint32_t)t;
         }
         const UpdateArgs a{m, v, me, ve, steps, (const float2*)scale, partials ? clip : nullptr, lr_device, b1, b2,

@@ -586,7 +586,7 @@ static int check_group_norm(const char* who, int dtype, int N, int64_t P, int C,
     if (N < 1 || P < 1 || C < 1) return fail(RAFTCORR_EINVAL, "%s: N, P, C must be positive (got %d, %lld, %d)", who, N, (long long)P, C);
     if (groups < 1 || C % groups) return fail(RAFTCORR_EINVAL, "%s: %d channels in %d groups", who, C, groups);
     if (P > 1 && row < C) return fail(RAFTCORR_EINVAL, "%s: rows of %d channels overlap (stride %lld)", who, C, (long long)row);
-    if (C > 1 << 20 || P > 1LL << 40 || (int64_t)N * ((C + 255) / 256) > kMostBlocks || (int64_t)N * groups / 4 + C / 4 + 1 > kMostBlocks)
+    if (C > 1 << 20 || P > 1LL << 40 || (int64_t)N * ((C + 255) / 256) > kMostBlocks || (int64_t)N * groups + C > kMostBlocks / 4)
         return fail(RAFTCORR_EUNSUPPORTED, "%s: N = %d, P = %lld, C = %d too large", who, N, (long long)P, C);
     if (!workspace || workspace_bytes < (int64_t)group_norm_workspace_bytes(N, C, groups))
         return fail(RAFTCORR_EINVAL, "%s: workspace of %lld bytes, need %lld", who, (long long)workspace_bytes,
@@ -601,19 +601,19 @@ int64_t raftcorr_group_norm_workspace_bytes(int N, int C, int groups)
 }
 
 int raftcorr_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int groups,
-                            const float* weight, const float* bias, double eps, int act, void* y, float* stats,
+                            const float* weight, const float* bias, double eps, int act, void* y, double* stats,
                             void* workspace, int64_t workspace_bytes, void* stream)
 {
     const int rc = check_group_norm("group_norm_fwd", dtype, N, P, C, groups, act, x_row, workspace_bytes, workspace);
     if (rc) return rc;
     if (!x || !y || !stats) return fail(RAFTCORR_EINVAL, "group_norm_fwd: null pointer");
     if (!(eps >= 0.0)) return fail(RAFTCORR_EINVAL, "group_norm_fwd: eps = %g", eps);
-    return launch_group_norm_fwd(x, x_batch, x_row, dtype, N, P, C, groups, weight, bias, (float)eps, act, y, stats, workspace, (hipStream_t)stream);
+    return launch_group_norm_fwd(x, x_batch, x_row, dtype, N, P, C, groups, weight, bias, eps, act, y, stats, workspace, (hipStream_t)stream);
 }
 
 int raftcorr_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t dy_batch, int64_t dy_row,
                             int dtype, int N, int64_t P, int C, int groups, const float* weight, const float* bias, int act,
-                            const float* stats, void* dx, float* dweight, float* dbias,
+                            const double* stats, void* dx, float* dweight, float* dbias,
                             void* workspace, int64_t workspace_bytes, void* stream)
 {
     const int rc = check_group_norm("group_norm_bwd", dtype, N, P, C, groups, act, x_row < dy_row ? x_row : dy_row, workspace_bytes, workspace);
@@ -667,7 +667,7 @@ int raftcorr_adamw_step(void* const* params, const void* const* grads, const int
     if (!offsets || !slots || !exp_avg || !exp_avg_sq || !steps || !scale || (state_bits == 8 && (!exp_avg_exp || !exp_avg_sq_exp)))
         return fail(RAFTCORR_EINVAL, "adamw_step: null pointer");
     for (int i = 0; i < count; ++i)
-        if (offsets[i] < 0 || offsets[i] % RAFTCORR_ADAMW_TILE || offsets[i] / RAFTCORR_ADAMW_TILE > 0xFFFFFFFFLL || slots[i] < 0)
+        if (offsets[i] < 0 || offsets[i] % RAFTCORR_ADAMW_TILE || offsets[i] / RAFTCORR_ADAMW_TILE > 0xFFFFFFFFLL || slots[i] < 0 || slots[i] >= 1 << 22)
             return fail(RAFTCORR_EINVAL, "adamw_step: tensor %d has offset %lld, slot %d", i, (long long)offsets[i], slots[i]);
     if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 && weight_decay >= 0.0) || (!lr_device && !(lr >= 0.0)))
         return fail(RAFTCORR_EINVAL, "adamw_step: lr = %g, betas = (%g, %g), eps = %g, weight_decay = %g", lr, beta1, beta2, eps, weight_decay);

@@ -89,9 +89,9 @@ int launch_alt_lookup_bwd16(const void* f1t, const void* const* f2t, const float
 
 size_t group_norm_workspace_bytes(int N, int C, int G);
 int launch_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int G, const float* w,
-                          const float* b, float eps, int act, void* y, float* stats, void* workspace, hipStream_t s);
+                          const float* b, double eps, int act, void* y, double* stats, void* workspace, hipStream_t s);
 int launch_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t d_batch, int64_t d_row, int dtype, int N,
-                          int64_t P, int C, int G, const float* w, const float* b, int act, const float* stats, void* dx, float* dw,
+                          int64_t P, int C, int G, const float* w, const float* b, int act, const double* stats, void* dx, float* dw,
                           float* db, void* workspace, hipStream_t s);
 int64_t adamw_norm_partials(const int64_t* numels, int count);
 int launch_adamw_norm(const void* const* grads, const int64_t* numels, int count, int dtype, double* partial, hipStream_t s);

@@ -5,8 +5,11 @@
 //   xh = (x - mean) * rstd,  z = xh * w[c] + b[c],  y = act(z)
 //   g = dy * act'(z):  db[c] = sum g,  dw[c] = sum g * xh,
 //   dx = rstd * (g * w - s1 - xh * s2),  s1 = mean over the group of g * w,  s2 = mean over the group of g * w * xh.
-// Memory bound: 8 operations a value forward, some 20 backward.  Three launches each: sums of row ranges per channel, one small
-// launch that joins them per group, one pass that writes.
+// Memory bound: 8 operations a value forward, some 20 backward.
+// A workgroup that can hold all rows of a sample's channel slab in registers reads them once and does everything in one launch.
+// Else there are three: sums of row ranges per channel, one small launch that joins them per group, one pass that writes.  That
+// pass reads x again out of the 256 MB last-level cache as far as it fits; it loads and stores past the replacement order, so the
+// results do not displace what is still to be read (12 x 64 x 200 x 360 float32, forward: 75 us that pass without it, 65 with).
 #include "common.h"
 #include "elem.h"
 
@@ -26,7 +29,17 @@ struct NormGeom {
     int64_t rows;                // rows of a range
 };
 
-enum { kThreads = 256, kUnroll = 8 };
+enum {
+    kThreads = 256,
+    kWaves = 4,                  // workgroups a CU (registers: 128 a thread)
+    kUnroll = 4,                 // vectors of x that a thread has on their way at once, forward
+    kMostRanges = 1024,          // workgroups of a pass over everything ...
+    kFewRanges = 512,            // ... and while a range stays below kRangeBytes: each workgroup costs a launch, its coefficients and a join
+    kRangeBytes = 256 << 10,     // (2 x 64 x 220 x 512 float32, forward: 512 take 34 us, 1024 36; 12 x 64 x 200 x 360: 117 and 109)
+};
+
+// the same backward, of x and of dy each
+template <int V> constexpr int unroll_bwd() { return V == 8 ? 2 : 4; }
 
 static int gcd_(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
@@ -36,7 +49,10 @@ static void slab_geom(NormGeom& g, int V)
     const int pattern = g.C / gcd_(g.C, V);          // threads after which the channel pattern repeats
     if (pattern <= kThreads) {
         g.Cs = g.C; g.nslab = 1;
-        g.T = kThreads / pattern * pattern;
+        // 8 vectors of 16 bytes are a line: rounds of whole lines, or two rounds would each write a part of one
+        // (96 channels in 16 bits, 2 x 272 x 480: the writing pass takes 18 us with 240 threads, 21 with 252)
+        const int lines = pattern * (8 / gcd_(pattern, 8));
+        g.T = lines <= kThreads ? kThreads / lines * lines : kThreads / pattern * pattern;
     } else {
         g.Cs = V * kThreads; g.nslab = (g.C + g.Cs - 1) / g.Cs;
         g.T = kThreads;
@@ -53,22 +69,39 @@ template <int V> __device__ __forceinline__ void slab_of(const NormGeom& g, int 
     if (cs != g.Cs) { const int cols = cs / V; R = kThreads / cols; T = R * cols; }   // last slab: V divides its width (or V == 1)
 }
 
-// sum over the row lanes of NQ quantities a slot: slot f = t * V + j of thread t holds channel f % cs, row lane f / cs.
-// buf: NQ * kThreads * V floats; afterwards buf[q * kThreads * V + c] is channel c's sum.  Fixed order.
-template <int V, int NQ> __device__ __forceinline__ void reduce_columns(float (&val)[NQ][V], float* buf, int T, int R, int cs)
+// Row lane, channel and group of each of a thread's V slots (slot j: value t * V + j of a round), by one division each and counting.
+template <int V> struct Slots {
+    int lane[V], c[V], group[V];
+    int col;                                         // first slot's column in the slab
+    __device__ __forceinline__ Slots(const NormGeom& g, int t, int c0, int cs)
+    {
+        const unsigned f = (unsigned)t * V;
+        int l = (int)(f / (unsigned)cs), k = (int)(f % (unsigned)cs);
+        col = k;
+        int p = (int)((unsigned)(c0 + k) / (unsigned)g.D), rest = (c0 + k) - p * g.D;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            lane[j] = l; c[j] = c0 + k; group[j] = p;
+            ++k; ++rest;
+            if (rest == g.D) { rest = 0; ++p; }
+            if (k == cs) { k = 0; ++l; rest = 0; p = 0; }            // only where the slab is the whole row: from channel 0 again
+        }
+    }
+};
+
+// sum over the row lanes of a quantity of each slot: slot f = t * V + j of thread t holds channel f % cs, row lane f / cs.
+// buf: blockDim * V values; afterwards buf[c] is channel c's sum.  Fixed order.
+template <int V, typename S> __device__ __forceinline__ void reduce_columns(const S (&val)[V], S* buf, int T, int R, int cs)
 {
     const int t = threadIdx.x;
     __syncthreads();
     if (t < T)
-        for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int j = 0; j < V; ++j) buf[q * kThreads * V + t * V + j] = val[q][j];
+        for (int j = 0; j < V; ++j) buf[t * V + j] = val[j];
     for (int rows = R; rows > 1;) {
         const int half = (rows + 1) / 2;
         __syncthreads();
-        for (int f = t; f < (rows - half) * cs; f += kThreads)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) buf[q * kThreads * V + f] += buf[q * kThreads * V + f + half * cs];
+        for (int f = t; f < (rows - half) * cs; f += blockDim.x) buf[f] += buf[f + half * cs];
         rows = half;
     }
     __syncthreads();
@@ -76,125 +109,110 @@ template <int V, int NQ> __device__ __forceinline__ void reduce_columns(float (&
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
 
-// mean and sum of squared deviations of each channel over one row range -> part[n][s][c].  A thread takes 8 rows at a time (two
-// passes over them in registers) and joins the result with what it has: no sum of squares that a large mean would cancel.
+// Sum and sum of squares of each channel over one row range -> part[n][s][c].  In 64 bits (full rate here, three operations a value):
+// no mean is large enough to cancel the squares, and the statistics are exact enough for ReLU's gradient to tell on which side of
+// zero each z lies (see NormCoef).
 template <typename T_, int V>
-__global__ __launch_bounds__(kThreads) void norm_stats_kernel(const T_* __restrict__ x, NormGeom g, float2* __restrict__ part)
+__global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* __restrict__ x, NormGeom g, double2* __restrict__ part)
 {
-    __shared__ float buf[2 * kThreads * V];
+    constexpr int U = kUnroll;
+    __shared__ double buf[kThreads * V];
     const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
     const int64_t n = blockIdx.x / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
-    const int64_t r0 = s * g.rows, r1 = min(g.P, r0 + g.rows);
-    float mean[1][V] = {}, m2[1][V] = {};
-    int cnt[V];
-    int lane[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) { lane[j] = (t * V + j) / cs; cnt[j] = 0; }
+    const int64_t r1 = min(g.P, (s + 1) * g.rows);
+    double sum[V] = {}, squares[V] = {};
     if (t < T) {
+        const Slots<V> q(g, t, c0, cs);
+        const int (&lane)[V] = q.lane;
+        auto add = [&](T_ e, int j) {
+            const double d = (double)to_float(e);
+            sum[j] += d;
+            squares[j] += d * d;
+        };
         const int64_t step = (int64_t)R * g.x_row;
-        const T_* p = x + n * g.x_batch + (r0 + lane[0]) * g.x_row + c0 + (t * V) % cs;
-        int64_t r = r0;
-        int k = 0;
-        for (; r + (int64_t)kUnroll * R <= r1; r += kUnroll * R) {
-            Vec<T_, V> v[kUnroll];
+        int64_t r = s * g.rows;
+        const T_* p = x + n * g.x_batch + (r + lane[0]) * g.x_row + c0 + q.col;
+        for (; r + (int64_t)U * R <= r1; r += U * R) {
+            Vec<T_, V> v[U];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) { v[u] = load_vec<T_, V>(p); p += step; }
-            const float fa = (float)kUnroll / (float)(k + kUnroll), fb = fa * (float)k;
-            k += kUnroll;
+            for (int u = 0; u < U; ++u) { v[u] = load_vec<T_, V>(p); p += step; }
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float a = 0.f, q = 0.f;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) a += to_float(v[u][j]);
-                a *= 1.f / kUnroll;
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) { const float d = to_float(v[u][j]) - a; q += d * d; }
-                const float d = a - mean[0][j];
-                mean[0][j] += d * fa;
-                m2[0][j] += q + d * d * fb;
-            }
+                for (int j = 0; j < V; ++j) add(v[u][j], j);
         }
+        // what is left, all loads at once again; a vector that the range's end cuts comes value by value
+        Vec<T_, V> v[U];
 #pragma unroll
-        for (int j = 0; j < V; ++j) cnt[j] = k;
-        for (; r < r1; r += R) {
-            const float f = 1.f / (float)(k + 1);
-            ++k;
-            if (r + lane[V - 1] < r1) {
-                const Vec<T_, V> v = load_vec<T_, V>(p);
+        for (int u = 0; u < U; ++u)
+            if (r + u * R + lane[V - 1] < r1) v[u] = load_vec<T_, V>(p + u * step);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float d = to_float(v[j]) - mean[0][j];
-                    mean[0][j] += d * f;
-                    m2[0][j] += d * (to_float(v[j]) - mean[0][j]);
-                    cnt[j] = k;
-                }
-            } else {
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = r + u * R;
+            if (at + lane[V - 1] < r1) {
 #pragma unroll
+                for (int j = 0; j < V; ++j) add(v[u][j], j);
+            } else if (at + lane[0] < r1) {
                 for (int j = 0; j < V; ++j)
-                    if (r + lane[j] < r1) {
-                        const float e = to_float(p[j]), d = e - mean[0][j];
-                        mean[0][j] += d * f;
-                        m2[0][j] += d * (e - mean[0][j]);
-                        cnt[j] = k;
-                    }
+                    if (at + lane[j] < r1) add(p[u * step + j], j);
             }
-            p += step;
         }
     }
-    // join the row lanes: mean of the means, then the deviations around it
-    float w[1][V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) w[0][j] = mean[0][j] * (float)cnt[j];
-    reduce_columns<V, 1>(w, buf, T, R, cs);
-    float* keep = buf + kThreads * V;
-    const float inv = 1.f / (float)(r1 - r0);
-    for (int c = t; c < cs; c += kThreads) keep[c] = buf[c] * inv;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float d = t < T ? mean[0][j] - keep[(t * V + j) % cs] : 0.f;
-        w[0][j] = m2[0][j] + d * d * (float)cnt[j];
-    }
-    reduce_columns<V, 1>(w, buf, T, R, cs);
-    for (int c = t; c < cs; c += kThreads)
-        part[(n * g.S + s) * g.C + c0 + c] = make_float2(keep[c], buf[c]);
+    double2* out = part + (n * g.S + s) * g.C + c0;
+    reduce_columns<V>(sum, buf, T, R, cs);
+    for (int c = t; c < cs; c += kThreads) out[c].x = buf[c];
+    reduce_columns<V>(squares, buf, T, R, cs);
+    for (int c = t; c < cs; c += kThreads) out[c].y = buf[c];
 }
 
-__device__ __forceinline__ float wave_sum(float v)
+template <typename S> __device__ __forceinline__ S wave_sum(S v)
 {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
-// part -> (mean, rstd) of each (n, group); one wave each
-__global__ __launch_bounds__(kThreads) void norm_join_kernel(const float2* __restrict__ part, NormGeom g, float eps, float2* __restrict__ stats)
+// sum of v over the workgroup's threads (whole waves), in every thread; buf: one value a wave
+template <typename S> __device__ __forceinline__ S block_sum(S v, S* buf)
 {
-    const int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
-    if (i >= (int64_t)g.N * g.G) return;
-    const int64_t n = i / g.G;
-    const float2* p = part + n * g.S * g.C + i % g.G * g.D;
-    const int l = threadIdx.x & 63, count = g.S * g.D;
-    const float full = (float)g.rows, last = (float)(g.P - (g.S - 1) * g.rows);
-    float a = 0.f;
-    for (int k = l; k < count; k += 64) {
-        const int s = k / g.D;
-        a += p[(int64_t)s * g.C + k % g.D].x * (s == g.S - 1 ? last : full);
+    v = wave_sum(v);
+    const int waves = blockDim.x / 64;
+    if (waves == 1) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = buf[0];
+    for (int w = 1; w < waves; ++w) v += buf[w];
+    return v;
+}
+
+// (mean, rstd) from a group's sum and sum of squares, inv = 1 / (P D)
+__device__ __forceinline__ double2 statistics(double sum, double squares, double inv, double eps)
+{
+    const double mean = sum * inv, var = squares * inv - mean * mean;
+    return make_double2(mean, 1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps));       // (a NaN stays one)
+}
+
+// part -> (mean, rstd) of each (n, group); one workgroup each, so that all its reads are on their way at once
+__global__ __launch_bounds__(1024) void norm_join_kernel(const double2* __restrict__ part, NormGeom g, double eps, double2* __restrict__ stats)
+{
+    __shared__ double buf[16];
+    const int64_t n = blockIdx.x / (unsigned)g.G;
+    const double2* p = part + n * g.S * g.C + (int64_t)(blockIdx.x % (unsigned)g.G) * g.D;
+    const unsigned count = (unsigned)g.S * g.D, D = g.D;
+    double a = 0.0, q = 0.0;
+#pragma unroll 4
+    for (unsigned k = threadIdx.x; k < count; k += blockDim.x) {
+        const double2 v = p[(int64_t)(k / D) * g.C + k % D];
+        a += v.x;
+        q += v.y;
     }
-    const float inv = 1.f / ((float)g.P * (float)g.D);
-    const float mean = wave_sum(a) * inv;
-    float q = 0.f;
-    for (int k = l; k < count; k += 64) {
-        const int s = k / g.D;
-        const float2 v = p[(int64_t)s * g.C + k % g.D];
-        const float d = v.x - mean;
-        q += v.y + d * d * (s == g.S - 1 ? last : full);
-    }
-    const float var = wave_sum(q) * inv;
-    if (l == 0) stats[i] = make_float2(mean, 1.f / sqrtf(var + eps));
+    a = block_sum(a, buf);
+    q = block_sum(q, buf);
+    if (threadIdx.x == 0) stats[blockIdx.x] = statistics(a, q, 1.0 / ((double)g.P * (double)g.D), eps);
 }
 
 template <int ACT> __device__ __forceinline__ float activate(float z)
@@ -206,7 +224,6 @@ template <int ACT> __device__ __forceinline__ float activate(float z)
 
 template <int ACT> __device__ __forceinline__ float slope(float z)
 {
-    if (ACT == RAFTCORR_ACT_RELU) return z > 0.f ? 1.f : 0.f;
     if (ACT == RAFTCORR_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.f + expf(-z));
         return s * (1.f + z * (1.f - s));
@@ -215,10 +232,11 @@ template <int ACT> __device__ __forceinline__ float slope(float z)
 }
 
 template <typename T_, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T_* __restrict__ x, NormGeom g, const float2* __restrict__ stats,
+__global__ __launch_bounds__(kThreads, kWaves) void norm_apply_kernel(const T_* __restrict__ x, NormGeom g, const double2* __restrict__ stats,
                                                               const float* __restrict__ weight, const float* __restrict__ bias,
                                                               T_* __restrict__ y)
 {
+    constexpr int U = kUnroll;
     const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
     const int64_t n = blockIdx.x / g.S / g.nslab;
     int c0, cs, T, R;
@@ -227,97 +245,127 @@ __global__ __launch_bounds__(kThreads) void norm_apply_kernel(const T_* __restri
     if (t >= T) return;
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
     float mean[V], a[V], b[V];
-    int lane[V];
+    const Slots<V> q(g, t, c0, cs);
+    const int (&lane)[V] = q.lane;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        lane[j] = (t * V + j) / cs;
-        const int c = c0 + (t * V + j) % cs;
-        const float2 st = stats[n * g.G + c / g.D];
-        mean[j] = st.x;
-        a[j] = weight ? st.y * weight[c] : st.y;
+        const int c = q.c[j];
+        const double2 st = stats[n * g.G + q.group[j]];
+        mean[j] = (float)st.x;
+        a[j] = (float)st.y * (weight ? weight[c] : 1.f);
         b[j] = bias ? bias[c] : 0.f;
     }
     const int64_t step = (int64_t)R * g.x_row, ystep = (int64_t)R * g.C;
-    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + (t * V) % cs;
-    T_* o = y + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + (t * V) % cs;
+    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col;
+    T_* o = y + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + q.col;
     int64_t r = s * g.rows;
-    for (; r + (int64_t)kUnroll * R <= r1; r += kUnroll * R) {
-        Vec<T_, V> v[kUnroll];
+    for (; r + (int64_t)U * R <= r1; r += U * R) {
+        Vec<T_, V> v[U];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) { v[u] = load_vec<T_, V>(p); p += step; }
+        for (int u = 0; u < U; ++u) { v[u] = load_vec_once<T_, V>(p); p += step; }
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             Vec<T_, V> w;
 #pragma unroll
             for (int j = 0; j < V; ++j) w[j] = from_float<T_>(activate<ACT>((to_float(v[u][j]) - mean[j]) * a[j] + b[j]));
-            store_vec<T_, V>(o, w);
+            store_vec_once<T_, V>(o, w);
             o += ystep;
         }
     }
-    for (; r < r1; r += R) {
-        if (r + lane[V - 1] < r1) {
-            const Vec<T_, V> v = load_vec<T_, V>(p);
+    Vec<T_, V> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (r + u * R + lane[V - 1] < r1) v[u] = load_vec_once<T_, V>(p + u * step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = r + u * R;
+        if (at + lane[V - 1] < r1) {
             Vec<T_, V> w;
 #pragma unroll
-            for (int j = 0; j < V; ++j) w[j] = from_float<T_>(activate<ACT>((to_float(v[j]) - mean[j]) * a[j] + b[j]));
-            store_vec<T_, V>(o, w);
-        } else {
+            for (int j = 0; j < V; ++j) w[j] = from_float<T_>(activate<ACT>((to_float(v[u][j]) - mean[j]) * a[j] + b[j]));
+            store_vec_once<T_, V>(o + u * ystep, w);
+        } else if (at + lane[0] < r1) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (r + lane[j] < r1) o[j] = from_float<T_>(activate<ACT>((to_float(p[j]) - mean[j]) * a[j] + b[j]));
+                if (at + lane[j] < r1) o[u * ystep + j] = from_float<T_>(activate<ACT>((to_float(p[u * step + j]) - mean[j]) * a[j] + b[j]));
         }
-        p += step;
-        o += ystep;
     }
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 
-// what a slot needs of its channel
-struct NormCoef { float mean, rstd, w, b; };
+// What a slot needs of its channel.  ReLU passes a gradient where z = (x - mean) rstd w + b > 0, that is where x is above (for w < 0:
+// below) the point mean - b / (rstd w).  That point is computed in 64 bits and rounded down to a float32 `edge`, and x, with its
+// sign turned for w < 0, is compared with it: the right side for every x, one operation instead of two.  With z in float32 one in
+// some 10^8 values would land on the wrong side, and its whole gradient with it.
+struct NormCoef { float mean, rstd, w, b, turn, edge; };
 
-__device__ __forceinline__ NormCoef coef_of(const NormGeom& g, const float2* stats, const float* weight, const float* bias, int64_t n, int c)
+__device__ __forceinline__ float round_down(double d)
 {
-    const float2 st = stats[n * g.G + c / g.D];
-    return NormCoef{st.x, st.y, weight ? weight[c] : 1.f, bias ? bias[c] : 0.f};
+    const float f = (float)d;
+    if (!((double)f > d)) return f;
+    const uint32_t u = __float_as_uint(f);
+    return __uint_as_float(f > 0.f ? u - 1 : f < 0.f ? u + 1 : 0x80000001u);
+}
+
+template <int ACT>
+__device__ __forceinline__ NormCoef coef_of(double2 st, const float* weight, const float* bias, int c)
+{
+    NormCoef k{(float)st.x, (float)st.y, weight ? weight[c] : 1.f, bias ? bias[c] : 0.f, 1.f, 0.f};
+    if (ACT == RAFTCORR_ACT_RELU) {
+        k.turn = k.w < 0.f ? -1.f : 1.f;
+        const double scale = (double)k.w * st.y;
+        double r = __builtin_amdgcn_rcp(scale);             // two Newton steps: 64 bits (half the instructions of a division)
+        r = fma(r, fma(-scale, r, 1.0), r);
+        r = fma(r, fma(-scale, r, 1.0), r);
+        const double at = st.x - (k.b != 0.f ? (double)k.b * r : 0.0);
+        k.edge = k.w == 0.f ? (k.b > 0.f ? -__builtin_inff() : __builtin_inff()) : round_down(k.turn * at);
+    }
+    return k;
+}
+
+// g = dy * act'(z)
+template <int ACT> __device__ __forceinline__ float through(const NormCoef& k, float x, float xh, float dy)
+{
+    if (ACT == RAFTCORR_ACT_RELU) return x * k.turn > k.edge ? dy : 0.f;
+    return dy * slope<ACT>(xh * k.w + k.b);
 }
 
 // sum of g and of g * xh of each channel over one row range -> part[n][s][c]
 template <typename T_, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(const T_* __restrict__ x, const T_* __restrict__ dy, NormGeom g,
-                                                                 const float2* __restrict__ stats, const float* __restrict__ weight,
+__global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_sums_kernel(const T_* __restrict__ x, const T_* __restrict__ dy, NormGeom g,
+                                                                 const double2* __restrict__ stats, const float* __restrict__ weight,
                                                                  const float* __restrict__ bias, float2* __restrict__ part)
 {
-    __shared__ float buf[2 * kThreads * V];
+    constexpr int U = unroll_bwd<V>();
+    __shared__ float buf[kThreads * V];
     const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
     const int64_t n = blockIdx.x / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
-    float sum[2][V] = {};
+    float sum[V] = {}, dot[V] = {};
     if (t < T) {
         NormCoef k[V];
-        int lane[V];
+        const Slots<V> q(g, t, c0, cs);
+        const int (&lane)[V] = q.lane;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            lane[j] = (t * V + j) / cs;
-            k[j] = coef_of(g, stats, weight, bias, n, c0 + (t * V + j) % cs);
-        }
+        for (int j = 0; j < V; ++j) k[j] = coef_of<ACT>(stats[n * g.G + q.group[j]], weight, bias, q.c[j]);
         auto add = [&](float xv, float dv, int j, float& a, float& b) {
             const float xh = (xv - k[j].mean) * k[j].rstd;
-            const float e = dv * slope<ACT>(xh * k[j].w + k[j].b);
+            const float e = through<ACT>(k[j], xv, xh, dv);
             a += e;
             b += e * xh;
         };
         const int64_t step = (int64_t)R * g.x_row, dstep = (int64_t)R * g.d_row;
-        const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + (t * V) % cs;
-        const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + (t * V) % cs;
+        const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col;
+        const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + q.col;
         int64_t r = s * g.rows;
-        for (; r + (int64_t)(kUnroll / 2) * R <= r1; r += kUnroll / 2 * R) {
-            Vec<T_, V> v[kUnroll / 2], w[kUnroll / 2];
+        for (; r + (int64_t)U * R <= r1; r += U * R) {
+            Vec<T_, V> v[U], w[U];
 #pragma unroll
-            for (int u = 0; u < kUnroll / 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 v[u] = load_vec<T_, V>(p); p += step;
                 w[u] = load_vec<T_, V>(d); d += dstep;
             }
@@ -325,76 +373,88 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_sums_kernel(const T_* __res
             for (int j = 0; j < V; ++j) {
                 float a = 0.f, b = 0.f;                      // the chunk by itself first: long sums lose less
 #pragma unroll
-                for (int u = 0; u < kUnroll / 2; ++u) add(to_float(v[u][j]), to_float(w[u][j]), j, a, b);
-                sum[0][j] += a;
-                sum[1][j] += b;
+                for (int u = 0; u < U; ++u) add(to_float(v[u][j]), to_float(w[u][j]), j, a, b);
+                sum[j] += a;
+                dot[j] += b;
             }
         }
-        for (; r < r1; r += R) {
-            if (r + lane[V - 1] < r1) {
-                const Vec<T_, V> v = load_vec<T_, V>(p), w = load_vec<T_, V>(d);
+        Vec<T_, V> v[U], w[U];
 #pragma unroll
-                for (int j = 0; j < V; ++j) add(to_float(v[j]), to_float(w[j]), j, sum[0][j], sum[1][j]);
-            } else {
+        for (int u = 0; u < U; ++u)
+            if (r + u * R + lane[V - 1] < r1) {
+                v[u] = load_vec<T_, V>(p + u * step);
+                w[u] = load_vec<T_, V>(d + u * dstep);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t at = r + u * R;
+            if (at + lane[V - 1] < r1) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) add(to_float(v[u][j]), to_float(w[u][j]), j, sum[j], dot[j]);
+            } else if (at + lane[0] < r1) {
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (r + lane[j] < r1) add(to_float(p[j]), to_float(d[j]), j, sum[0][j], sum[1][j]);
+                    if (at + lane[j] < r1) add(to_float(p[u * step + j]), to_float(d[u * dstep + j]), j, sum[j], dot[j]);
             }
-            p += step;
-            d += dstep;
         }
     }
-    reduce_columns<V, 2>(sum, buf, T, R, cs);
-    for (int c = t; c < cs; c += kThreads)
-        part[(n * g.S + s) * g.C + c0 + c] = make_float2(buf[c], buf[kThreads * V + c]);
+    float2* out = part + (n * g.S + s) * g.C + c0;
+    reduce_columns<V>(sum, buf, T, R, cs);
+    for (int c = t; c < cs; c += kThreads) out[c].x = buf[c];
+    reduce_columns<V>(dot, buf, T, R, cs);
+    for (int c = t; c < cs; c += kThreads) out[c].y = buf[c];
 }
 
-// part -> (s1, s2) of each (n, group) and, with dweight / dbias, the channels' sums over all samples; one wave each
-__global__ __launch_bounds__(kThreads) void norm_bwd_join_kernel(const float2* __restrict__ part, NormGeom g, const float* __restrict__ weight,
-                                                                 float2* __restrict__ coef, float* __restrict__ dweight, float* __restrict__ dbias)
+// part -> (s1, s2) of each (n, group) and, in further workgroups with dweight / dbias, a channel's sums over all samples
+__global__ __launch_bounds__(1024) void norm_bwd_join_kernel(const float2* __restrict__ part, NormGeom g, const float* __restrict__ weight,
+                                                             float2* __restrict__ coef, float* __restrict__ dweight, float* __restrict__ dbias)
 {
-    int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
-    const int l = threadIdx.x & 63;
+    __shared__ float buf[16];
+    const unsigned T = blockDim.x, groups = (unsigned)g.N * g.G;
     float a = 0.f, b = 0.f;
-    if (i < (int64_t)g.N * g.G) {
-        const int64_t n = i / g.G;
-        const int c0 = (int)(i % g.G) * g.D;
-        for (int64_t k = l; k < (int64_t)g.S * g.D; k += 64) {
-            const int c = c0 + (int)(k % g.D);
-            const float2 v = part[(n * g.S + k / g.D) * g.C + c];
-            const float w = weight ? weight[c] : 1.f;
+    if (blockIdx.x < groups) {
+        const int c0 = (int)(blockIdx.x % (unsigned)g.G) * g.D;
+        const float2* p = part + (int64_t)(blockIdx.x / (unsigned)g.G) * g.S * g.C + c0;
+        const unsigned count = (unsigned)g.S * g.D, D = g.D;
+#pragma unroll 4
+        for (unsigned k = threadIdx.x; k < count; k += T) {
+            const unsigned c = k % D;
+            const float2 v = p[(int64_t)(k / D) * g.C + c];
+            const float w = weight ? weight[c0 + c] : 1.f;
             a += v.x * w;
             b += v.y * w;
         }
         const float inv = 1.f / ((float)g.P * (float)g.D);
-        a = wave_sum(a) * inv;
-        b = wave_sum(b) * inv;
-        if (l == 0) coef[i] = make_float2(a, b);
+        a = block_sum(a, buf) * inv;
+        b = block_sum(b, buf) * inv;
+        if (threadIdx.x == 0) coef[blockIdx.x] = make_float2(a, b);
         return;
     }
-    i -= (int64_t)g.N * g.G;
-    if (i >= g.C || !(dweight || dbias)) return;
-    for (int64_t k = l; k < (int64_t)g.N * g.S; k += 64) {
-        const float2 v = part[k * g.C + i];
+    const unsigned c = blockIdx.x - groups;
+#pragma unroll 4
+    for (int64_t k = threadIdx.x; k < (int64_t)g.N * g.S; k += T) {
+        const float2 v = part[k * g.C + c];
         a += v.x;
         b += v.y;
     }
-    a = wave_sum(a);
-    b = wave_sum(b);
-    if (l == 0) {
-        if (dbias) dbias[i] = a;
-        if (dweight) dweight[i] = b;
+    a = block_sum(a, buf);
+    b = block_sum(b, buf);
+    if (threadIdx.x == 0) {
+        if (dbias) dbias[c] = a;
+        if (dweight) dweight[c] = b;
     }
 }
 
 template <typename T_, int V, int ACT>
-__global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(const T_* __restrict__ x, const T_* __restrict__ dy, NormGeom g,
-                                                                  const float2* __restrict__ stats, const float* __restrict__ weight,
+__global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_apply_kernel(const T_* __restrict__ x, const T_* __restrict__ dy, NormGeom g,
+                                                                  const double2* __restrict__ stats, const float* __restrict__ weight,
                                                                   const float* __restrict__ bias, const float2* __restrict__ coef,
-                                                                  T_* __restrict__ dx)
+                                                                  T_* __restrict__ dx, int backwards)
 {
-    const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
-    const int64_t n = blockIdx.x / g.S / g.nslab;
+    constexpr int U = unroll_bwd<V>();
+    const unsigned block = backwards ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int s = block % g.S, slab = block / g.S % g.nslab;
+    const int64_t n = block / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
@@ -402,56 +462,227 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_apply_kernel(const T_* __re
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
     NormCoef k[V];
     float2 m[V];
-    int lane[V];
+    const Slots<V> q(g, t, c0, cs);
+    const int (&lane)[V] = q.lane;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        lane[j] = (t * V + j) / cs;
-        const int c = c0 + (t * V + j) % cs;
-        k[j] = coef_of(g, stats, weight, bias, n, c);
-        m[j] = coef[n * g.G + c / g.D];
+        k[j] = coef_of<ACT>(stats[n * g.G + q.group[j]], weight, bias, q.c[j]);
+        m[j] = coef[n * g.G + q.group[j]];
     }
     auto grad = [&](float xv, float dv, int j) {
         const float xh = (xv - k[j].mean) * k[j].rstd;
-        const float e = dv * slope<ACT>(xh * k[j].w + k[j].b);
+        const float e = through<ACT>(k[j], xv, xh, dv);
         return k[j].rstd * (e * k[j].w - m[j].x - xh * m[j].y);
     };
     const int64_t step = (int64_t)R * g.x_row, dstep = (int64_t)R * g.d_row, ostep = (int64_t)R * g.C;
-    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + (t * V) % cs;
-    const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + (t * V) % cs;
-    T_* o = dx + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + (t * V) % cs;
+    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col;
+    const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + q.col;
+    T_* o = dx + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + q.col;
     int64_t r = s * g.rows;
-    for (; r + (int64_t)(kUnroll / 2) * R <= r1; r += kUnroll / 2 * R) {
-        Vec<T_, V> v[kUnroll / 2], w[kUnroll / 2];
+    for (; r + (int64_t)U * R <= r1; r += U * R) {
+        Vec<T_, V> v[U], w[U];
 #pragma unroll
-        for (int u = 0; u < kUnroll / 2; ++u) {
-            v[u] = load_vec<T_, V>(p); p += step;
-            w[u] = load_vec<T_, V>(d); d += dstep;
+        for (int u = 0; u < U; ++u) {
+            v[u] = load_vec_once<T_, V>(p); p += step;
+            w[u] = load_vec_once<T_, V>(d); d += dstep;
         }
 #pragma unroll
-        for (int u = 0; u < kUnroll / 2; ++u) {
-            Vec<T_, V> q;
+        for (int u = 0; u < U; ++u) {
+            Vec<T_, V> f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) q[j] = from_float<T_>(grad(to_float(v[u][j]), to_float(w[u][j]), j));
-            store_vec<T_, V>(o, q);
+            for (int j = 0; j < V; ++j) f[j] = from_float<T_>(grad(to_float(v[u][j]), to_float(w[u][j]), j));
+            store_vec_once<T_, V>(o, f);
             o += ostep;
         }
     }
-    for (; r < r1; r += R) {
-        if (r + lane[V - 1] < r1) {
-            const Vec<T_, V> v = load_vec<T_, V>(p), w = load_vec<T_, V>(d);
-            Vec<T_, V> q;
+    Vec<T_, V> v[U], w[U];
 #pragma unroll
-            for (int j = 0; j < V; ++j) q[j] = from_float<T_>(grad(to_float(v[j]), to_float(w[j]), j));
-            store_vec<T_, V>(o, q);
-        } else {
+    for (int u = 0; u < U; ++u)
+        if (r + u * R + lane[V - 1] < r1) {
+            v[u] = load_vec_once<T_, V>(p + u * step);
+            w[u] = load_vec_once<T_, V>(d + u * dstep);
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = r + u * R;
+        if (at + lane[V - 1] < r1) {
+            Vec<T_, V> f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[j] = from_float<T_>(grad(to_float(v[u][j]), to_float(w[u][j]), j));
+            store_vec_once<T_, V>(o + u * ostep, f);
+        } else if (at + lane[0] < r1) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (r + lane[j] < r1) o[j] = from_float<T_>(grad(to_float(p[j]), to_float(d[j]), j));
+                if (at + lane[j] < r1) o[u * ostep + j] = from_float<T_>(grad(to_float(p[u * step + j]), to_float(d[u * dstep + j]), j));
         }
-        p += step;
-        d += dstep;
-        o += ostep;
     }
+}
+
+
+// ---- small: one workgroup holds a slab of whole groups of one sample --------------------------------------------------------
+
+// Slab of a workgroup: whole groups, whole vectors, 32 or 64 bytes of each row at least.  T threads, K rounds.
+struct SmallGeom { int Cs, nslab, T, K; };
+
+// most threads of such a workgroup: the slots' sums take 32 KB
+template <int V> constexpr int small_threads() { return V == 8 ? 512 : 1024; }
+// of the variant with K rounds: the largest K only come with 256
+template <int V, int K, bool BACKWARD> constexpr int small_bound() { return K > (BACKWARD ? 4 : 8) ? 256 : small_threads<V>(); }
+
+// sum over each group's channels of buf[c] (times weight[c]) / count -> out[group]: a thread a group of few channels, a wave a larger one
+template <typename S> __device__ __forceinline__ void small_groups(const S* buf, const float* weight, S inv, S* out, int cs, int D)
+{
+    if (D <= 16) {
+        for (int k = threadIdx.x; k < cs / D; k += blockDim.x) {
+            S a = 0;
+            for (int c = k * D; c < k * D + D; ++c) a += buf[c] * (weight ? weight[c] : 1.f);
+            out[k] = a * inv;
+        }
+    } else {
+        const int l = threadIdx.x & 63;
+        for (int k = threadIdx.x / 64; k < cs / D; k += blockDim.x / 64) {
+            S a = 0;
+            for (int c = l; c < D; c += 64) a += buf[k * D + c] * (weight ? weight[k * D + c] : 1.f);
+            a = wave_sum(a) * inv;
+            if (l == 0) out[k] = a;
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T_, int V, int ACT, int K>
+__global__ __launch_bounds__((small_bound<V, K, false>())) void norm_small_kernel(const T_* __restrict__ x, NormGeom g, const float* __restrict__ weight,
+                                                                        const float* __restrict__ bias, double eps, T_* __restrict__ y,
+                                                                        double2* __restrict__ stats)
+{
+    extern __shared__ double small_buf[];              // blockDim * V slots, then two values a group
+    double* buf = small_buf;
+    const int64_t n = blockIdx.x / (unsigned)g.nslab;
+    const int c0 = (int)(blockIdx.x % (unsigned)g.nslab) * g.Cs, cs = min(g.Cs, g.C - c0), cols = cs / V;
+    const int R = blockDim.x / cols, T = R * cols, t = threadIdx.x, P = (int)g.P;
+    double* group_mean = buf + blockDim.x * V;
+    double* group_rstd = group_mean + g.Cs / g.D;
+    const int r0 = t / cols, c = t % cols * V;          // the thread's first row and its channels in the slab
+    const bool work = t < T;
+    Vec<T_, V> v[K];
+    const T_* p = x + n * g.x_batch + r0 * g.x_row + c0 + c;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (work && r0 + k * R < P) v[k] = load_vec<T_, V>(p + (int64_t)k * R * g.x_row);
+    double sum[V] = {}, squares[V] = {};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (work && r0 + k * R < P)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double e = (double)to_float(v[k][j]);
+                sum[j] += e;
+                squares[j] += e * e;
+            }
+    reduce_columns<V>(sum, buf, T, R, cs);
+    small_groups(buf, nullptr, 1.0, group_mean, cs, g.D);
+    reduce_columns<V>(squares, buf, T, R, cs);
+    small_groups(buf, nullptr, 1.0, group_rstd, cs, g.D);
+    const double inv = 1.0 / ((double)P * (double)g.D);
+    for (int k = t; k < cs / g.D; k += blockDim.x) {
+        const double2 st = statistics(group_mean[k], group_rstd[k], inv, eps);
+        group_mean[k] = st.x;
+        group_rstd[k] = st.y;
+        stats[n * g.G + c0 / g.D + k] = st;
+    }
+    __syncthreads();
+    if (!work) return;
+    float mean[V], a[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        mean[j] = (float)group_mean[(c + j) / g.D];
+        a[j] = (float)group_rstd[(c + j) / g.D] * (weight ? weight[c0 + c + j] : 1.f);
+        b[j] = bias ? bias[c0 + c + j] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) keep_packed(v[k]);
+    T_* o = y + (n * P + r0) * g.C + c0 + c;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (r0 + k * R < P) {
+            Vec<T_, V> w;
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = from_float<T_>(activate<ACT>((to_float(v[k][j]) - mean[j]) * a[j] + b[j]));
+            store_vec<T_, V>(o + (int64_t)k * R * g.C, w);
+        }
+}
+
+// dx, and each channel's sums of g and g * xh over the sample -> part[n][c] (or, for one sample, dbias and dweight themselves)
+template <typename T_, int V, int ACT, int K>
+__global__ __launch_bounds__((small_bound<V, K, true>())) void norm_small_bwd_kernel(const T_* __restrict__ x, const T_* __restrict__ dy, NormGeom g,
+                                                              const double2* __restrict__ stats, const float* __restrict__ weight,
+                                                              const float* __restrict__ bias, T_* __restrict__ dx, float2* __restrict__ part,
+                                                              float* __restrict__ dweight, float* __restrict__ dbias)
+{
+    extern __shared__ double small_buf[];
+    float* buf = (float*)small_buf;
+    const int64_t n = blockIdx.x / (unsigned)g.nslab;
+    const int c0 = (int)(blockIdx.x % (unsigned)g.nslab) * g.Cs, cs = min(g.Cs, g.C - c0), cols = cs / V;
+    const int R = blockDim.x / cols, T = R * cols, t = threadIdx.x, P = (int)g.P;
+    float* s1 = buf + blockDim.x * V;
+    float* s2 = s1 + g.Cs / g.D;
+    const int r0 = t / cols, c = t % cols * V;
+    const bool work = t < T;
+    Vec<T_, V> v[K], d[K];
+    const T_* p = x + n * g.x_batch + r0 * g.x_row + c0 + c;
+    const T_* q = dy + n * g.d_batch + r0 * g.d_row + c0 + c;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (work && r0 + k * R < P) {
+            v[k] = load_vec<T_, V>(p + (int64_t)k * R * g.x_row);
+            d[k] = load_vec<T_, V>(q + (int64_t)k * R * g.d_row);
+        }
+    NormCoef e[V];
+    float a[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        a[j] = b[j] = 0.f;
+        e[j] = work ? coef_of<ACT>(stats[n * g.G + (c0 + c + j) / g.D], weight, bias, c0 + c + j) : NormCoef{};
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (work && r0 + k * R < P) {
+                const float xh = (to_float(v[k][j]) - e[j].mean) * e[j].rstd;
+                const float h = through<ACT>(e[j], to_float(v[k][j]), xh, to_float(d[k][j]));
+                a[j] += h;
+                b[j] += h * xh;
+            }
+    }
+    const float inv = 1.f / ((float)P * (float)g.D);
+    const float* w = weight ? weight + c0 : nullptr;
+    reduce_columns<V>(a, buf, T, R, cs);
+    for (int i = t; i < cs; i += blockDim.x) {
+        if (part) part[n * g.C + c0 + i].x = buf[i];
+        if (dbias) dbias[c0 + i] = buf[i];
+    }
+    small_groups(buf, w, inv, s1, cs, g.D);
+    reduce_columns<V>(b, buf, T, R, cs);
+    for (int i = t; i < cs; i += blockDim.x) {
+        if (part) part[n * g.C + c0 + i].y = buf[i];
+        if (dweight) dweight[c0 + i] = buf[i];
+    }
+    if (!dx) return;
+    small_groups(buf, w, inv, s2, cs, g.D);
+#pragma unroll
+    for (int k = 0; k < K; ++k) { keep_packed(v[k]); keep_packed(d[k]); }
+    if (!work) return;
+    T_* o = dx + (n * P + r0) * g.C + c0 + c;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (r0 + k * R < P) {
+            Vec<T_, V> f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (to_float(v[k][j]) - e[j].mean) * e[j].rstd;
+                const float h = through<ACT>(e[j], to_float(v[k][j]), xh, to_float(d[k][j]));
+                f[j] = from_float<T_>(e[j].rstd * (h * e[j].w - s1[(c + j) / g.D] - xh * s2[(c + j) / g.D]));
+            }
+            store_vec<T_, V>(o + (int64_t)k * R * g.C, f);
+        }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -468,49 +699,115 @@ static NormGeom norm_geom(int N, int64_t P, int C, int G, int64_t x_batch, int64
     V = dtype == RAFTCORR_DTYPE_FP32 ? 4 : 8;
     if (!full_vectors(g, V)) V = 1;
     slab_geom(g, V);
-    // some four workgroups a CU, each with one unrolled round at least
-    const int64_t most = (P + (int64_t)kUnroll * g.R - 1) / ((int64_t)kUnroll * g.R);
-    int64_t S = 1024 / ((int64_t)N * g.nslab);
+    const int64_t chunk = (int64_t)g.R * kUnroll, most = (P + chunk - 1) / chunk;
+    const int64_t bytes = (int64_t)N * P * C * (dtype == RAFTCORR_DTYPE_FP32 ? 4 : 2);
+    int64_t S = (bytes > (int64_t)kFewRanges * kRangeBytes ? kMostRanges : kFewRanges) / ((int64_t)N * g.nslab);
     S = S < 1 ? 1 : S > most ? most : S;
-    g.rows = ((P + S - 1) / S + g.R - 1) / g.R * g.R;
+    g.rows = (most + S - 1) / S * chunk;                 // whole rounds: only a sample's last range has a rest
     g.S = (int)((P + g.rows - 1) / g.rows);
     return g;
 }
 
-// The most row ranges any layout of these sizes is cut into: 1024 / N.
-static int64_t norm_part_bytes(int N, int C) { const int64_t S = 1024 / N; return (S < 1 ? 1 : S) * N * C * (int64_t)sizeof(float2); }
+// the most row ranges that any layout of these sizes is cut into
+static int64_t norm_part_bytes(int N, int C) { const int64_t S = kMostRanges / N; return (S < 1 ? 1 : S) * N * C * (int64_t)sizeof(double2); }
+
+// The one-launch form: K rounds of T threads hold P rows of a slab (K = 0: they do not).  A thread holds 16 vectors, forward of x and
+// backward 8 of x and 8 of dy; few threads with many vectors, whose sums take fewer steps to join, before many threads with half.
+static SmallGeom small_geom(const NormGeom& g, int V, int bytes, bool backward)
+{
+    SmallGeom q{};
+    const int unit = g.D / gcd_(g.D, V) * V;
+    if (g.C % V) return q;
+    // 32 bytes of a row while that makes few workgroups, else 64 (lines are fetched by fewer of them); forward and backward in us,
+    // 32 | 64: 64 channels x 500 rows float32 6.0, 8.9 | 6.3, 11.0; 12 x 96 x 25 x 45 float32 10.8, 18.6 | 10.1, 15.6
+    const int least = ((int64_t)g.N * g.C * bytes < 128 * 64 ? 32 : 64) / bytes;
+    q.Cs = unit * ((least + unit - 1) / unit);
+    if (q.Cs > g.C) q.Cs = g.C;
+    q.nslab = (g.C + q.Cs - 1) / q.Cs;
+    const int cols = q.Cs / V;
+    for (const int T : {256, V == 8 ? small_threads<8>() : small_threads<1>()}) {
+        if (cols > T) continue;
+        const int64_t K = (g.P + T / cols - 1) / (T / cols);
+        if (K <= (T == 256 ? 16 : 8) / (backward ? 2 : 1)) { q.T = T; q.K = K <= 2 ? 2 : K <= 4 ? 4 : K <= 8 ? 8 : 16; return q; }
+    }
+    return q;
+}
 
 size_t group_norm_workspace_bytes(int N, int C, int G) { return (size_t)(norm_part_bytes(N, C) + (int64_t)N * G * (int64_t)sizeof(float2)); }
 
-template <typename T_, int V>
-static void fwd_launch(const void* x, const NormGeom& g, const float* w, const float* b, float eps, int act, void* y, float2* stats, float2* part, hipStream_t s)
+// threads of a joining workgroup over `count` partial sums: whole waves, four values a thread while there are no more than 1024
+static unsigned join_threads(int64_t count)
 {
-    const unsigned blocks = (unsigned)((int64_t)g.N * g.nslab * g.S), joins = (unsigned)(((int64_t)g.N * g.G + 3) / 4);
+    const int64_t waves = (count + 255) / 256;
+    return 64 * (unsigned)(waves < 1 ? 1 : waves > 16 ? 16 : waves);
+}
+
+template <typename T_, int V, int ACT>
+static void small_fwd(const void* x, NormGeom g, const SmallGeom& q, const float* w, const float* b, double eps, void* y, double2* stats, hipStream_t s)
+{
+    g.Cs = q.Cs; g.nslab = q.nslab;
+    const unsigned blocks = (unsigned)((int64_t)g.N * q.nslab), lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(double));
+    if (q.K == 2) norm_small_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
+    else if (q.K == 4) norm_small_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
+    else if (q.K == 8) norm_small_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
+    else norm_small_kernel<T_, V, ACT, 16><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
+}
+
+template <typename T_, int V>
+static void fwd_launch(const void* x, const NormGeom& g, const float* w, const float* b, double eps, int act, void* y, double2* stats, double2* part, hipStream_t s)
+{
+    const SmallGeom q = small_geom(g, V, sizeof(T_), false);
+    if (q.K) {
+        if (act == RAFTCORR_ACT_RELU) small_fwd<T_, V, RAFTCORR_ACT_RELU>(x, g, q, w, b, eps, y, stats, s);
+        else if (act == RAFTCORR_ACT_SILU) small_fwd<T_, V, RAFTCORR_ACT_SILU>(x, g, q, w, b, eps, y, stats, s);
+        else small_fwd<T_, V, RAFTCORR_ACT_NONE>(x, g, q, w, b, eps, y, stats, s);
+        return;
+    }
+    const unsigned blocks = (unsigned)((int64_t)g.N * g.nslab * g.S), joins = (unsigned)((int64_t)g.N * g.G);
     norm_stats_kernel<T_, V><<<blocks, kThreads, 0, s>>>((const T_*)x, g, part);
-    norm_join_kernel<<<joins, kThreads, 0, s>>>(part, g, eps, stats);
+    norm_join_kernel<<<joins, join_threads((int64_t)g.S * g.D), 0, s>>>(part, g, eps, stats);
     if (act == RAFTCORR_ACT_RELU) norm_apply_kernel<T_, V, RAFTCORR_ACT_RELU><<<blocks, kThreads, 0, s>>>((const T_*)x, g, stats, w, b, (T_*)y);
     else if (act == RAFTCORR_ACT_SILU) norm_apply_kernel<T_, V, RAFTCORR_ACT_SILU><<<blocks, kThreads, 0, s>>>((const T_*)x, g, stats, w, b, (T_*)y);
     else norm_apply_kernel<T_, V, RAFTCORR_ACT_NONE><<<blocks, kThreads, 0, s>>>((const T_*)x, g, stats, w, b, (T_*)y);
 }
 
 template <typename T_, int V, int ACT>
-static void bwd_launch(const void* x, const void* dy, const NormGeom& g, const float* w, const float* b, const float2* stats, void* dx,
+static void bwd_launch(const void* x, const void* dy, const NormGeom& g, const float* w, const float* b, const double2* stats, void* dx,
                        float* dw, float* db, float2* part, float2* coef, hipStream_t s)
 {
+    const SmallGeom q = small_geom(g, V, sizeof(T_), true);
+    if (q.K) {
+        NormGeom h = g;
+        h.Cs = q.Cs; h.nslab = q.nslab; h.S = 1; h.rows = g.P;
+        const bool join = (dw || db) && g.N > 1;
+        const unsigned blocks = (unsigned)((int64_t)g.N * q.nslab), lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(float));
+        float2* sums = join ? part : nullptr;
+        float *dw1 = join ? nullptr : dw, *db1 = join ? nullptr : db;
+        if (q.K == 2) norm_small_bwd_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>((const T_*)x, (const T_*)dy, h, stats, w, b, (T_*)dx, sums, dw1, db1);
+        else if (q.K == 4) norm_small_bwd_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>((const T_*)x, (const T_*)dy, h, stats, w, b, (T_*)dx, sums, dw1, db1);
+        else norm_small_bwd_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>((const T_*)x, (const T_*)dy, h, stats, w, b, (T_*)dx, sums, dw1, db1);
+        h.G = 0;                                                       // the channels' sums alone
+        if (join) norm_bwd_join_kernel<<<g.C, join_threads(g.N), 0, s>>>(part, h, w, coef, dw, db);
+        return;
+    }
     const unsigned blocks = (unsigned)((int64_t)g.N * g.nslab * g.S);
-    const unsigned joins = (unsigned)(((int64_t)g.N * g.G + (dw || db ? g.C : 0) + 3) / 4);
+    const unsigned joins = (unsigned)((int64_t)g.N * g.G + (dw || db ? g.C : 0));
+    const int64_t most = (int64_t)g.S * g.D > (dw || db ? (int64_t)g.S * g.N : 0) ? (int64_t)g.S * g.D : (int64_t)g.S * g.N;
     norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>((const T_*)x, (const T_*)dy, g, stats, w, b, part);
-    norm_bwd_join_kernel<<<joins, kThreads, 0, s>>>(part, g, w, coef, dw, db);
-    if (dx) norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>((const T_*)x, (const T_*)dy, g, stats, w, b, coef, (T_*)dx);
+    norm_bwd_join_kernel<<<joins, join_threads(most), 0, s>>>(part, g, w, coef, dw, db);
+    const int backwards = 2 * g.N * g.P * g.C * (int64_t)sizeof(T_) > 256 << 20;
+    if (dx) norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>((const T_*)x, (const T_*)dy, g, stats, w, b, coef, (T_*)dx,
+                                                                               backwards);
 }
 
 int launch_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int G, const float* w,
-                          const float* b, float eps, int act, void* y, float* stats, void* workspace, hipStream_t s)
+                          const float* b, double eps, int act, void* y, double* stats, void* workspace, hipStream_t s)
 {
     int V;
     const NormGeom g = norm_geom(N, P, C, G, x_batch, x_row, x_batch, x_row, dtype, V);
-    float2* part = (float2*)workspace;
-    float2* st = (float2*)stats;
+    if (V > 1 && small_geom(g, 1, dtype == RAFTCORR_DTYPE_FP32 ? 4 : 2, false).K && C % V) V = 1;
+    double2* part = (double2*)workspace;
+    double2* st = (double2*)stats;
     if (dtype == RAFTCORR_DTYPE_FP32) {
         if (V == 4) fwd_launch<float, 4>(x, g, w, b, eps, act, y, st, part, s); else fwd_launch<float, 1>(x, g, w, b, eps, act, y, st, part, s);
     } else if (dtype == RAFTCORR_DTYPE_FP16) {
@@ -522,7 +819,7 @@ int launch_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dty
 }
 
 template <typename T_, int V>
-static void bwd_by_act(int act, const void* x, const void* dy, const NormGeom& g, const float* w, const float* b, const float2* stats, void* dx,
+static void bwd_by_act(int act, const void* x, const void* dy, const NormGeom& g, const float* w, const float* b, const double2* stats, void* dx,
                        float* dw, float* db, float2* part, float2* coef, hipStream_t s)
 {
     if (act == RAFTCORR_ACT_RELU) bwd_launch<T_, V, RAFTCORR_ACT_RELU>(x, dy, g, w, b, stats, dx, dw, db, part, coef, s);
@@ -531,14 +828,15 @@ static void bwd_by_act(int act, const void* x, const void* dy, const NormGeom& g
 }
 
 int launch_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t d_batch, int64_t d_row, int dtype, int N,
-                          int64_t P, int C, int G, const float* w, const float* b, int act, const float* stats, void* dx, float* dw,
+                          int64_t P, int C, int G, const float* w, const float* b, int act, const double* stats, void* dx, float* dw,
                           float* db, void* workspace, hipStream_t s)
 {
     int V;
     const NormGeom g = norm_geom(N, P, C, G, x_batch, x_row, d_batch, d_row, dtype, V);
+    if (V > 1 && small_geom(g, 1, dtype == RAFTCORR_DTYPE_FP32 ? 4 : 2, true).K && C % V) V = 1;
     float2* part = (float2*)workspace;
     float2* coef = (float2*)((char*)workspace + norm_part_bytes(N, C));
-    const float2* st = (const float2*)stats;
+    const double2* st = (const double2*)stats;
     if (dtype == RAFTCORR_DTYPE_FP32) {
         if (V == 4) bwd_by_act<float, 4>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
         else bwd_by_act<float, 1>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);

@@ -2,8 +2,12 @@
 
 Tolerances, u = 2^-24.  32-bit moments: the clipped gradient has two roundings (coefficient, product); the first moment adds
 its factor's, a product and the sum: 5 u of the terms' sizes.  The second squares the clipped gradient (four), and adds its factor's,
-two products and the sum: 8 u (float32's smallest step besides).  The update m / (sqrt(v) r + eps) has six more roundings, its factor two, the difference one: 16 u of the update's
-size plus 3 u of the parameter's.  bfloat16 parameters may be either neighbour of that.  8-bit moments are codes: those of the 64-bit
+two products and the sum: 8 u (float32's smallest step besides).  The update lr' m / (sqrt(v) r + eps) carries
+the first moment's 5 u (of its terms: they may cancel) and half the second's 8 u; the root and the reciprocal are instructions within
+a unit in the last place, 2 u each; r, its product, eps, the sum, the product with m, lr' and its product one u each: 4 + 2 + 2 + 7 = 15,
+taken as 16 u of the update's size, and 6 u of lr' (|b1 m| + |(1 - b1) g|) / (sqrt(v) r + eps).  The difference and the decay: 3 u of the
+parameter's.
+bfloat16 parameters may be either neighbour of that.  8-bit moments are codes: those of the 64-bit
 sums rounded to 32 bits, equal bit for bit (the kernel sums in 64 bits too)."""
 import copy
 import math
@@ -127,9 +131,10 @@ def check_step(opt, group_of=None, bits=32):
             assert np.array_equal(new["codes"][1], want[1][0]) and np.array_equal(new["codes"][3], want[1][1])
             m, v = m32.astype(np.float64), v32.astype(np.float64)
         with np.errstate(invalid="ignore"):
-            step = lr / (1 - b1 ** t) * m / (np.sqrt(v) / math.sqrt(1 - b2 ** t) + opts["eps"])
+            factor = lr / (1 - b1 ** t) / (np.sqrt(v) / math.sqrt(1 - b2 ** t) + opts["eps"])
+            step, terms = factor * m, factor * (np.abs(b1 * old["m"]) + np.abs((1 - b1) * e))
             value = old["p"] * (1 - lr * opts["weight_decay"]) - step
-            bound = 16 * U * np.abs(step) + 3 * U * (np.abs(old["p"]) + np.abs(value)) + 2.0 ** -148
+            bound = 16 * U * np.abs(step) + 6 * U * terms + 3 * U * (np.abs(old["p"]) + np.abs(value)) + 2.0 ** -148
             if p.dtype == torch.bfloat16:
                 bound = bound + np.abs(value) * 2.0 ** -7                    # one whole step: up or down
             off = np.abs(new["p"] - value)

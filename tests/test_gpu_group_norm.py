@@ -1,10 +1,10 @@
 """raft_amd.group_norm against the formula in 64 bits, forward and backward.
 
-Tolerances.  u = 2^-24.  A sum here is a tree: 8 rows in registers, at most 16 joins of a thread's own rounds at these sizes, 10
-levels over a workgroup's threads, at most 22 steps over row ranges and channels; with the roundings of the formula itself no
-value passes through more than 64.  So statistics are within 64 u of the mean size of what is summed, z within 64 u times
-(|xh| + |mean| rstd + 1) |w| + |b|, and a result of a 16-bit type is then rounded once (half a step, finfo.eps / 2).  Where |z| is
-below its own bound the slope of ReLU may be either side's, and the sums may have the value or not."""
+Tolerances.  u = 2^-24.  A gradient's sum here is a tree: 4 rows in registers, at most 16 joins of a thread's own rounds at these
+sizes, 10 levels over a workgroup's threads, at most 22 steps over row ranges and channels; with the roundings of the formula
+itself no value passes through more than 64.  The statistics are sums in 64 bits that are rounded once.  So z is within 64 u times
+(|xh| + |mean| rstd + 1) |w| + |b|, and a result of a 16-bit type is then rounded once (half a step, finfo.eps / 2).  ReLU's slope is
+that of z in 64 bits and has no tolerance."""
 import pytest
 import torch
 
@@ -38,8 +38,8 @@ def formula(x, w, b, groups, eps, act, dy):
         return (y, yt)
     d = dy.detach().cpu().double()
     slope = {"none": torch.ones_like(z), "relu": (z > 0).double(), "silu": s * (1 + z * (1 - s))}[act]
-    # an error of z moves the slope of silu by at most half of it; relu's is open where z is
-    st = {"none": torch.zeros_like(z), "relu": (z.abs() <= zt).double(), "silu": 0.5 * zt + U * (1 + z.abs())}[act]
+    # an error of z moves the slope of silu by at most half of it
+    st = {"none": torch.zeros_like(z), "relu": torch.zeros_like(z), "silu": 0.5 * zt + U * (1 + z.abs())}[act]
     xt = U * (2 * xh.abs() + shift + 1)
     g, gt = d * slope, d.abs() * st + U * (d * slope).abs()
     gw, gwt = g * wd, gt * wd.abs()
@@ -104,7 +104,8 @@ def check(dev, shape, groups, act="relu", dtype="fp32", affine=True, layout="las
 
 SIZES = [((1, 1, 1, 1), 1), ((2, 4, 1, 1), 2), ((3, 6, 2, 1), 6), ((1, 3, 5, 7), 1), ((2, 3, 9, 31), 3), ((2, 8, 13, 17), 8), ((1, 42, 19, 23), 7),
          ((2, 96, 25, 40), 96), ((1, 64, 55, 128), 8), ((3, 33, 31, 33), 11), ((1, 257, 9, 11), 257), ((2, 260, 12, 7), 4), ((1, 1030, 5, 9), 2),
-         ((1, 2050, 3, 5), 41), ((1, 4104, 3, 5), 3), ((1, 8, 300, 301), 1), ((130, 16, 3, 3), 4), ((1300, 5, 2, 3), 5)]
+         ((2, 42, 61, 67), 7), ((1, 1030, 40, 41), 5), ((1, 2056, 43, 21), 257), ((5, 3, 71, 73), 1), ((1, 96, 111, 65), 96), ((9, 16, 64, 64), 2),
+         ((3, 512, 1, 1), 1), ((70, 24, 8, 9), 24), ((2, 64, 32, 32), 64), ((1, 8200, 2, 3), 5), ((1, 2050, 3, 5), 41), ((1, 4104, 3, 5), 3), ((1, 8, 300, 301), 1), ((130, 16, 3, 3), 4), ((1300, 5, 2, 3), 5)]
 
 
 @pytest.mark.parametrize("shape,groups", SIZES, ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else f"g{v}")
@@ -141,6 +142,38 @@ def test_large_means_do_not_cancel(dev):
     """mean / width = 1000: with sums of squares in float32 the variance would have no digit left."""
     check(dev, (2, 16, 60, 61), 4, "none", shift=1000.0, seed=4)
     check(dev, (1, 64, 130, 131), 64, "none", affine=False, shift=1000.0, seed=5)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("shape", [(2, 16, 6, 7), (1, 16, 90, 91)], ids=str)
+def test_relu_takes_the_side_of_the_exact_value(dev, dtype, shape):
+    """A bias that puts the zero of z a few units of 2^-24 from many of the values, above and below, for weights of both signs and of
+    zero: what passes the gradient on is decided as in 64 bits."""
+    from raft_amd import group_norm
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(shape, generator=g).to(DTYPES[dtype]).to(dev)
+    x = x.contiguous(memory_format=torch.channels_last)
+    xd = x.double().cpu()
+    per = xd.reshape(shape[0], 4, -1)
+    mean, var = per.mean(2), per.var(2, unbiased=False)
+    rstd = ((var + 1e-5) ** -0.5).repeat_interleave(4, 1)
+    mean = mean.repeat_interleave(4, 1)
+    w = torch.randn(16, generator=g)
+    w[3] = 0.0
+    b = torch.empty(16)
+    for c in range(16):                                   # the zero close to one of the channel's values
+        b[c] = -(xd[0, c, 3, 4] - mean[0, c]) * rstd[0, c] * w[c]
+    b = b * (1 + (torch.arange(16) % 5 - 2) * 2.0 ** -23)
+    b[3] = 0.25
+    z = (xd - mean[:, :, None, None]) * rstd[:, :, None, None] * w.double().view(1, -1, 1, 1) + b.double().view(1, -1, 1, 1)
+    for whole in (False, True):                           # d(bias) counts the values that pass: the one at the border, and all of them
+        dy = torch.ones_like(x) if whole else torch.zeros_like(x)
+        dy[0, :, 3, 4] = 1.0
+        leaf = b.to(dev).requires_grad_(True)
+        y = group_norm(x, 4, w.to(dev), leaf, activation="relu")
+        db, = torch.autograd.grad(y, leaf, dy)
+        want = ((z > 0).double() * dy.double().cpu()).sum((0, 2, 3))
+        assert torch.equal(db.double().cpu(), want), db.cpu() - want
 
 
 def test_constant_groups(dev):
