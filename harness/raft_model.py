@@ -12,6 +12,8 @@ architecture and the parameter names follow the reference so that its checkpoint
   RAFT-small (RAFT(..., small=True)): core/raft.py:31-35,50-53 (hidden 96, context 64, radius 3, 128-channel features),
   bottleneck encoder core/extractor_origin.py:58-113,192-263, motion encoder + ConvGRU core/update.py:16-31,62-77,99-112,
   bilinear x8 upsampling instead of the convex mask (core/raft.py:135-136)
+`fused_norm=True` runs the encoders' instance / group norms with the ReLU behind them as raft_amd.GroupNorm, the encoders in
+torch.channels_last; parameter names and checkpoints stay the same.
 The model never imports a correlation implementation: `corr_factory(fmap1, fmap2)` must return a
 callable `coords (B,2,H/8,W/8) -> (B, 4*81, H/8, W/8)` (raft_amd.CorrBlock, raft_amd.AlternateCorrBlock,
 or the oracle's restatement of the reference).
@@ -24,9 +26,16 @@ CORR_LEVELS, CORR_RADIUS = 4, 4          # core/raft.py:40-41
 HIDDEN, CONTEXT = 128, 128               # core/raft.py:38-39
 
 
-def _norm(kind, ch):
+def _norm(kind, ch, fused=False, activation="relu"):
+    """core/extractor_origin.py:16-38: the four kinds (group norm with 8 channels a group).  fused: instance and group norm as
+    raft_amd.GroupNorm, which then holds the activation too."""
+    if fused and kind in ("instance", "group"):
+        from raft_amd import GroupNorm
+        return GroupNorm(ch if kind == "instance" else ch // 8, ch, affine=kind == "group", activation=activation)
     if kind == "instance":
         return nn.InstanceNorm2d(ch)
+    if kind == "group":
+        return nn.GroupNorm(ch // 8, ch)
     if kind == "batch":
         return nn.BatchNorm2d(ch)
     if kind == "none":
@@ -34,20 +43,25 @@ def _norm(kind, ch):
     raise ValueError(kind)
 
 
+def _norm_relu(norm, x):
+    y = norm(x)
+    return y if getattr(norm, "activation", None) == "relu" else F.relu(y)
+
+
 class ResidualBlock(nn.Module):
-    def __init__(self, cin, cout, norm, stride):
+    def __init__(self, cin, cout, norm, stride, fused=False):
         super().__init__()
         self.conv1 = nn.Conv2d(cin, cout, 3, padding=1, stride=stride)
         self.conv2 = nn.Conv2d(cout, cout, 3, padding=1)
-        self.norm1, self.norm2 = _norm(norm, cout), _norm(norm, cout)
+        self.norm1, self.norm2 = _norm(norm, cout, fused), _norm(norm, cout, fused)
         self.downsample = None
         if stride != 1:
-            self.norm3 = _norm(norm, cout)
+            self.norm3 = _norm(norm, cout, fused, "none")
             self.downsample = nn.Sequential(nn.Conv2d(cin, cout, 1, stride=stride), self.norm3)
 
     def forward(self, x):
-        y = F.relu(self.norm1(self.conv1(x)))
-        y = F.relu(self.norm2(self.conv2(y)))
+        y = _norm_relu(self.norm1, self.conv1(x))
+        y = _norm_relu(self.norm2, self.conv2(y))
         if self.downsample is not None:
             x = self.downsample(x)
         return F.relu(x + y)
@@ -56,25 +70,30 @@ class ResidualBlock(nn.Module):
 class BasicEncoder(nn.Module):
     """1/8-resolution encoder: 7x7 s2 stem, three 2-block stages (64, 96 s2, 128 s2), 1x1 head."""
 
-    def __init__(self, output_dim, norm):
+    def __init__(self, output_dim, norm, fused=False):
         super().__init__()
         self.conv1 = nn.Conv2d(3, 64, 7, stride=2, padding=3)
-        self.norm1 = _norm(norm, 64)
+        self.norm1 = _norm(norm, 64, fused)
         widths, strides, cin = (64, 96, 128), (1, 2, 2), 64
         for i, (w, s) in enumerate(zip(widths, strides), start=1):
-            setattr(self, f"layer{i}", nn.Sequential(ResidualBlock(cin, w, norm, s), ResidualBlock(w, w, norm, 1)))
+            setattr(self, f"layer{i}", nn.Sequential(ResidualBlock(cin, w, norm, s, fused), ResidualBlock(w, w, norm, 1, fused)))
             cin = w
         self.conv2 = nn.Conv2d(128, output_dim, 1)
         for m in self.modules():
             if isinstance(m, nn.Conv2d):
                 nn.init.kaiming_normal_(m.weight, mode="fan_out", nonlinearity="relu")
+        self.fused = fused
+        if fused:
+            self.to(memory_format=torch.channels_last)
 
     def forward(self, x):
         pair = isinstance(x, (tuple, list))
         if pair:
             n = x[0].shape[0]
             x = torch.cat(x, 0)
-        x = F.relu(self.norm1(self.conv1(x)))
+        if self.fused:
+            x = x.contiguous(memory_format=torch.channels_last)
+        x = _norm_relu(self.norm1, self.conv1(x))
         x = self.conv2(self.layer3(self.layer2(self.layer1(x))))
         return torch.split(x, [n, n], 0) if pair else x
 
@@ -82,22 +101,22 @@ class BasicEncoder(nn.Module):
 class Bottleneck(nn.Module):
     """1x1 (to a quarter of the width) -> 3x3 (carries the stride) -> 1x1, residual."""
 
-    def __init__(self, cin, cout, norm, stride):
+    def __init__(self, cin, cout, norm, stride, fused=False):
         super().__init__()
         mid = cout // 4
         self.conv1 = nn.Conv2d(cin, mid, 1)
         self.conv2 = nn.Conv2d(mid, mid, 3, padding=1, stride=stride)
         self.conv3 = nn.Conv2d(mid, cout, 1)
-        self.norm1, self.norm2, self.norm3 = _norm(norm, mid), _norm(norm, mid), _norm(norm, cout)
+        self.norm1, self.norm2, self.norm3 = _norm(norm, mid, fused), _norm(norm, mid, fused), _norm(norm, cout, fused)
         self.downsample = None
         if stride != 1:
-            self.norm4 = _norm(norm, cout)
+            self.norm4 = _norm(norm, cout, fused, "none")
             self.downsample = nn.Sequential(nn.Conv2d(cin, cout, 1, stride=stride), self.norm4)
 
     def forward(self, x):
-        y = F.relu(self.norm1(self.conv1(x)))
-        y = F.relu(self.norm2(self.conv2(y)))
-        y = F.relu(self.norm3(self.conv3(y)))
+        y = _norm_relu(self.norm1, self.conv1(x))
+        y = _norm_relu(self.norm2, self.conv2(y))
+        y = _norm_relu(self.norm3, self.conv3(y))
         if self.downsample is not None:
             x = self.downsample(x)
         return F.relu(x + y)
@@ -106,25 +125,30 @@ class Bottleneck(nn.Module):
 class SmallEncoder(nn.Module):
     """1/8-resolution encoder of RAFT-small: 7x7 s2 stem (32), three 2-bottleneck stages (32, 64 s2, 96 s2), 1x1 head."""
 
-    def __init__(self, output_dim, norm):
+    def __init__(self, output_dim, norm, fused=False):
         super().__init__()
         self.conv1 = nn.Conv2d(3, 32, 7, stride=2, padding=3)
-        self.norm1 = _norm(norm, 32)
+        self.norm1 = _norm(norm, 32, fused)
         cin = 32
         for i, (w, s) in enumerate(zip((32, 64, 96), (1, 2, 2)), start=1):
-            setattr(self, f"layer{i}", nn.Sequential(Bottleneck(cin, w, norm, s), Bottleneck(w, w, norm, 1)))
+            setattr(self, f"layer{i}", nn.Sequential(Bottleneck(cin, w, norm, s, fused), Bottleneck(w, w, norm, 1, fused)))
             cin = w
         self.conv2 = nn.Conv2d(96, output_dim, 1)
         for m in self.modules():
             if isinstance(m, nn.Conv2d):
                 nn.init.kaiming_normal_(m.weight, mode="fan_out", nonlinearity="relu")
+        self.fused = fused
+        if fused:
+            self.to(memory_format=torch.channels_last)
 
     def forward(self, x):
         pair = isinstance(x, (tuple, list))
         if pair:
             n = x[0].shape[0]
             x = torch.cat(x, 0)
-        x = F.relu(self.norm1(self.conv1(x)))
+        if self.fused:
+            x = x.contiguous(memory_format=torch.channels_last)
+        x = _norm_relu(self.norm1, self.conv1(x))
         x = self.conv2(self.layer3(self.layer2(self.layer1(x))))
         return torch.split(x, [n, n], 0) if pair else x
 
@@ -270,23 +294,24 @@ def upflow8(flow):
 
 
 class RAFT(nn.Module):
-    def __init__(self, corr_factory, fuse_convc1=False, small=False):
+    def __init__(self, corr_factory, fuse_convc1=False, small=False, fused_norm=False):
         """fuse_convc1: the correlation block must offer lookup_conv1x1 (differentiable)
         (raft_amd.CorrBlock does): the motion encoder's first 1x1 conv + ReLU then runs inside
         the lookup kernel and the (B, 324, H, W) tensor is never materialised.
-        small: RAFT-small -- the factory must build a radius-3 block on 128-channel features."""
+        small: RAFT-small -- the factory must build a radius-3 block on 128-channel features.
+        fused_norm: the feature encoder's norms and ReLUs as raft_amd.GroupNorm, channels last (CUDA only)."""
         super().__init__()
         self.corr_factory = corr_factory
         self.fuse_convc1 = fuse_convc1
         self.small = small
         if small:
             self.hidden, self.context = 96, 64
-            self.fnet = SmallEncoder(128, "instance")
+            self.fnet = SmallEncoder(128, "instance", fused_norm)
             self.cnet = SmallEncoder(self.hidden + self.context, "none")
             self.update_block = SmallUpdateBlock(radius=3, hidden=self.hidden)
         else:
             self.hidden, self.context = HIDDEN, CONTEXT
-            self.fnet = BasicEncoder(256, "instance")
+            self.fnet = BasicEncoder(256, "instance", fused_norm)
             self.cnet = BasicEncoder(HIDDEN + CONTEXT, "batch")
             self.update_block = BasicUpdateBlock()
 

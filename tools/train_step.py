@@ -8,6 +8,9 @@ and runs on RCCL over xGMI (backend "nccl").  The reference uses single-process 
 (train.py:342), which is not replicated.
 
     python tools/train_step.py [--steps K] [--warmup W] [--corr ours|ours_fused|stock|alt] [--batch 6] [--iters 12]
+                               [--norm stock|fused] [--optim stock|fused|fused8]
+--norm fused: the feature encoder's norms as raft_amd.GroupNorm.  --optim fused / fused8: raft_amd.AdamW with the gradient clipping
+inside, moments in 32 / 8 bits.
     python -m torch.distributed.run --nnodes=1 --nproc-per-node N --master-addr 127.0.0.1 \
            --master-port P tools/train_step.py ...
 Prints one JSON line from rank 0: image pairs/s over all ranks, ms per step, and the share of the
@@ -45,6 +48,8 @@ def main():
     ap.add_argument("--iters", type=int, default=12)
     ap.add_argument("--size", type=int, nargs=2, default=[400, 720])
     ap.add_argument("--device", default="cuda")
+    ap.add_argument("--norm", default="stock", choices=["stock", "fused"])
+    ap.add_argument("--optim", default="stock", choices=["stock", "fused", "fused8"])
     args = ap.parse_args()
 
     rank, world = int(os.environ.get("RANK", "0")), int(os.environ.get("WORLD_SIZE", "1"))
@@ -61,12 +66,16 @@ def main():
     torch.manual_seed(0)                                   # identical initial weights on every rank
     # ours_fused: lookup fused with the motion encoder's convc1 + ReLU (differentiable, raft_amd/corr.py:_LookupConv)
     model = RAFT(corr_factory("ours" if args.corr == "ours_fused" else args.corr),
-                 fuse_convc1=args.corr == "ours_fused").to(dev).train()
+                 fuse_convc1=args.corr == "ours_fused", fused_norm=args.norm == "fused").to(dev).train()
     for m in model.modules():                              # freeze_bn (core/raft.py:60-63), as every stage after chairs
         if isinstance(m, nn.BatchNorm2d):
             m.eval()
     net = nn.parallel.DistributedDataParallel(model, device_ids=[local] if on_gpu else None) if world > 1 else model
-    opt = torch.optim.AdamW(net.parameters(), lr=2e-4, weight_decay=5e-5, eps=1e-8)
+    if args.optim == "stock":
+        opt = torch.optim.AdamW(net.parameters(), lr=2e-4, weight_decay=5e-5, eps=1e-8)
+    else:
+        from raft_amd import AdamW
+        opt = AdamW(net.parameters(), lr=2e-4, weight_decay=5e-5, eps=1e-8, state_bits=8 if args.optim == "fused8" else 32, max_norm=1.0)
     sched = torch.optim.lr_scheduler.StepLR(opt, round(100000 * 0.8))
     i1, i2, gt = synthetic_pair(args.batch, *args.size, seed=100 + rank, device=dev)   # each rank its own shard
     valid = torch.ones_like(gt[:, 0])
@@ -81,7 +90,8 @@ def main():
         opt.zero_grad(set_to_none=True)
         loss, metrics = sequence_loss(net(i1, i2, iters=args.iters), gt, valid)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(net.parameters(), 1.0)
+        if args.optim == "stock":
+            torch.nn.utils.clip_grad_norm_(net.parameters(), 1.0)
         opt.step()
         sched.step()
         return float(loss.detach())
@@ -100,7 +110,7 @@ def main():
     if rank == 0:
         print(json.dumps({"metric": "training image pairs/sec (RAFT-basic, synthetic FlyingThings crops)",
                           "value": world * args.steps * args.batch / el, "n_gpus": world, "ms_per_step": el / args.steps * 1e3,
-                          "steps": args.steps, "warmup": args.warmup, "corr": args.corr, "batch_per_gpu": args.batch,
+                          "steps": args.steps, "warmup": args.warmup, "corr": args.corr, "norm": args.norm, "optim": args.optim, "batch_per_gpu": args.batch,
                           "iters": args.iters, "crop": args.size, "final_loss": loss, "scaling": "weak",
                           "collective": "DDP gradient all-reduce, 5257536 fp32" if world > 1 else None}), flush=True)
     if dist is not None:
