@@ -390,7 +390,7 @@ int raftcorr_alt_features_bwd(const float* d1, const float* const* d2_levels, in
  * relu'(0) = 0, and ReLU's side is that of z in 64 bits.  Statistics are summed in float64, gradients in float32; no atomics, the same
  * bits on every call.  x, dy, y, dx need no more than their
  * element's alignment.  Any C, groups that divide it, P, N >= 1; row stride >= C unless P == 1.
- * RAFTCORR_EUNSUPPORTED where N * groups + C passes 2^22 or C passes 2^20. */
+ * No buffer that is written may overlap another.  RAFTCORR_EUNSUPPORTED where C passes 2^20 or P 2^40. */
 #define RAFTCORR_ACT_NONE 0
 #define RAFTCORR_ACT_RELU 1
 #define RAFTCORR_ACT_SILU 2
@@ -418,7 +418,7 @@ int raftcorr_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const
  * Clipping: raftcorr_adamw_norm leaves raftcorr_adamw_norm_partials(numels, count) float64 sums of squares in `partial`; the sums
  * of all tensors that share the norm stand one behind the other (`partials` of them) when raftcorr_adamw_step is called, which
  * writes the norm to `norm` (float32) and the coefficient to `clip` (float64).  partials == 0: no clipping, these may be NULL.
- * Gradients stay as they are.  Two calls give the same bits.
+ * Gradients stay as they are.  Two calls give the same bits.  RAFTCORR_EUNSUPPORTED: a tensor of more than 2^34 values.
  * raftcorr_adamw_decode writes 8-bit moments as numbers (FP32, or BF16, which holds the codes' four digits exactly from 2^-126 up). */
 #define RAFTCORR_ADAMW_TILE  512
 #define RAFTCORR_ADAMW_BLOCK 64

@@ -108,6 +108,8 @@ class AdamW(torch.optim.Optimizer):
             made.append([])
             for params in by_kind.values():
                 made[-1].append(_Bucket(params, bits, sum(map(len, made))))
+        if _lib.glue().Bucket.overlap([p for buckets in made for b in buckets for p in b.params]):
+            raise RuntimeError("two parameters share memory (or one is listed twice)")
         for buckets in made:
             for b in buckets:
                 for i, p in enumerate(b.params):

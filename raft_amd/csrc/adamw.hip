@@ -364,6 +364,14 @@ __global__ __launch_bounds__(kWg) void adamw_decode_kernel(const uint8_t* __rest
 
 static int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
+// how many tensors from the i-th on one launch takes, and their tiles: `most` of them, less than 2^32 threads
+static int launch_share(const int64_t* numels, int i, int count, int most, int64_t& tiles)
+{
+    int n = 0;
+    for (tiles = 0; i + n < count && n < most && tiles + tiles_of(numels[i + n]) < 1 << 26; ++n) tiles += tiles_of(numels[i + n]);
+    return n;
+}
+
 // neighbouring tiles a wave of the norm pass takes: some 2048 workgroups, whole rounds of loads
 static uint32_t norm_run(int64_t tiles)
 {
@@ -376,11 +384,9 @@ int64_t adamw_norm_partials(const int64_t* numels, int count)
 {
     int64_t blocks = 0;
     for (int i = 0; i < count;) {
-        int64_t tiles = 0;
-        const int n = count - i < kNormTensors ? count - i : kNormTensors;
-        for (int k = 0; k < n; ++k) tiles += tiles_of(numels[i + k]);
+        int64_t tiles;
+        i += launch_share(numels, i, count, kNormTensors, tiles);
         blocks += norm_blocks(tiles);
-        i += n;
     }
     return blocks;
 }
@@ -390,7 +396,8 @@ int launch_adamw_norm(const void* const* grads, const int64_t* numels, int count
     for (int i = 0; i < count;) {
         NormTable tab;
         uint32_t tiles = 0;
-        const int n = count - i < kNormTensors ? count - i : kNormTensors;
+        int64_t all;
+        const int n = launch_share(numels, i, count, kNormTensors, all);
         for (int k = 0; k < n; ++k) {
             const int64_t t = tiles_of(numels[i + k]);
             tab.grad[k] = grads[i + k];
@@ -422,7 +429,8 @@ int launch_adamw_step(void* const* params, const void* const* grads, const int64
     for (int i = 0; i < count;) {
         UpdateTable tab;
         uint32_t tiles = 0;
-        const int n = count - i < kUpdateTensors ? count - i : kUpdateTensors;
+        int64_t all;
+        const int n = launch_share(numels, i, count, kUpdateTensors, all);
         for (int k = 0; k < n; ++k) {
             const int64_t t = tiles_of(numels[i + k]);
             tab.p[k] = (uint64_t)params[i + k];

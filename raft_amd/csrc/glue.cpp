@@ -4,6 +4,8 @@
 // function; reading the addresses of 124 parameters and gradients takes 75 us in Python.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
 #include "../../include/raftcorr.h"
@@ -140,6 +142,17 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     }
 };
 
+// A backward pass inside a capture ends the process where a leaf's accumulation node belongs to another stream, which it does while an
+// eager graph of the leaf is alive: refused before anything is recorded.
+void check_capture(const char* name, const Tensor& t)
+{
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (stream && *stream != c10::Stream(c10::hip::getCurrentHIPStream(t.device().index())))
+        REFUSE("group_norm: an eager graph of " << name << " is alive (on another stream than the capture's); delete its results before the capture");
+}
+
 Tensor group_norm(const Tensor& x, int64_t groups, const Maybe& weight_, const Maybe& bias_, double eps, int64_t act)
 {
     if (!x.is_cuda()) REFUSE("x must be a CUDA tensor");
@@ -157,7 +170,15 @@ Tensor group_norm(const Tensor& x, int64_t groups, const Maybe& weight_, const M
         *t = (*t)->to(at::kFloat).contiguous();
     }
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
+    {
+        const c10::OptionalDeviceGuard guard(x.device());
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+            check_capture("x", x);
+            check_capture("weight", weight_.value_or(Tensor()));
+            check_capture("bias", bias_.value_or(Tensor()));
+        }
         return GroupNorm::apply(x, weight, bias, groups, eps, act);
+    }
     return norm_forward(x, weight.value_or(Tensor()), bias.value_or(Tensor()), groups, eps, act).y;
 }
 
@@ -205,6 +226,18 @@ struct Bucket {
             strides.push_back(t.strides().vec());
             total += (t.numel() + RAFTCORR_ADAMW_TILE - 1) / RAFTCORR_ADAMW_TILE * RAFTCORR_ADAMW_TILE;
         }
+    }
+
+    // whether any two of all parameters share memory: they would be updated at the same time
+    static bool overlap(const std::vector<Tensor>& params)
+    {
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+        for (const Tensor& t : params)
+            if (t.numel()) spans.emplace_back((uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.numel() * t.element_size());
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second) return true;
+        return false;
     }
 
     // the addresses of the parameters that have a gradient; how many
@@ -272,6 +305,7 @@ PYBIND11_MODULE(_glue, m)
     m.def("same_order", [](const Tensor& a, const Tensor& b) { return same_order(a.sizes(), a.strides(), b.strides()); });
     py::class_<Bucket>(m, "Bucket")
         .def(py::init<const std::vector<Tensor>&>())
+        .def_static("overlap", &Bucket::overlap)
         .def_readonly("total", &Bucket::total)
         .def_readonly("offsets", &Bucket::offset)
         .def_readonly("numels", &Bucket::numel)

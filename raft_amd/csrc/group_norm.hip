@@ -12,6 +12,7 @@
 // results do not displace what is still to be read (12 x 64 x 200 x 360 float32, forward: 75 us that pass without it, 65 with).
 #include "common.h"
 #include "elem.h"
+#include <type_traits>
 
 namespace raftcorr {
 
@@ -27,6 +28,7 @@ struct NormGeom {
     int T, R;                    // threads at work, rows an iteration (first slabs)
     int S;                       // row ranges a sample is split into
     int64_t rows;                // rows of a range
+    int n0, n1;                  // first sample and samples of a launch
 };
 
 enum {
@@ -118,7 +120,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* 
     constexpr int U = kUnroll;
     __shared__ double buf[kThreads * V];
     const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
-    const int64_t n = blockIdx.x / g.S / g.nslab;
+    const int64_t n = g.n0 + blockIdx.x / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
@@ -200,8 +202,9 @@ __device__ __forceinline__ double2 statistics(double sum, double squares, double
 __global__ __launch_bounds__(1024) void norm_join_kernel(const double2* __restrict__ part, NormGeom g, double eps, double2* __restrict__ stats)
 {
     __shared__ double buf[16];
-    const int64_t n = blockIdx.x / (unsigned)g.G;
-    const double2* p = part + n * g.S * g.C + (int64_t)(blockIdx.x % (unsigned)g.G) * g.D;
+    const int64_t n = g.n0 + blockIdx.x / (unsigned)g.G;
+    const unsigned group = blockIdx.x % (unsigned)g.G;
+    const double2* p = part + n * g.S * g.C + (int64_t)group * g.D;
     const unsigned count = (unsigned)g.S * g.D, D = g.D;
     double a = 0.0, q = 0.0;
 #pragma unroll 4
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double2* __restri
     }
     a = block_sum(a, buf);
     q = block_sum(q, buf);
-    if (threadIdx.x == 0) stats[blockIdx.x] = statistics(a, q, 1.0 / ((double)g.P * (double)g.D), eps);
+    if (threadIdx.x == 0) stats[n * g.G + group] = statistics(a, q, 1.0 / ((double)g.P * (double)g.D), eps);
 }
 
 template <int ACT> __device__ __forceinline__ float activate(float z)
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_apply_kernel(const T_* 
 {
     constexpr int U = kUnroll;
     const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
-    const int64_t n = blockIdx.x / g.S / g.nslab;
+    const int64_t n = g.n0 + blockIdx.x / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
@@ -340,7 +343,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_sums_kernel(const T
     constexpr int U = unroll_bwd<V>();
     __shared__ float buf[kThreads * V];
     const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
-    const int64_t n = blockIdx.x / g.S / g.nslab;
+    const int64_t n = g.n0 + blockIdx.x / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
@@ -410,11 +413,13 @@ __global__ __launch_bounds__(1024) void norm_bwd_join_kernel(const float2* __res
                                                              float2* __restrict__ coef, float* __restrict__ dweight, float* __restrict__ dbias)
 {
     __shared__ float buf[16];
-    const unsigned T = blockDim.x, groups = (unsigned)g.N * g.G;
+    const unsigned T = blockDim.x, groups = (unsigned)g.n1 * g.G;
     float a = 0.f, b = 0.f;
     if (blockIdx.x < groups) {
-        const int c0 = (int)(blockIdx.x % (unsigned)g.G) * g.D;
-        const float2* p = part + (int64_t)(blockIdx.x / (unsigned)g.G) * g.S * g.C + c0;
+        const int64_t n = g.n0 + blockIdx.x / (unsigned)g.G;
+        const unsigned group = blockIdx.x % (unsigned)g.G;
+        const int c0 = (int)group * g.D;
+        const float2* p = part + n * g.S * g.C + c0;
         const unsigned count = (unsigned)g.S * g.D, D = g.D;
 #pragma unroll 4
         for (unsigned k = threadIdx.x; k < count; k += T) {
@@ -427,7 +432,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_join_kernel(const float2* __res
         const float inv = 1.f / ((float)g.P * (float)g.D);
         a = block_sum(a, buf) * inv;
         b = block_sum(b, buf) * inv;
-        if (threadIdx.x == 0) coef[blockIdx.x] = make_float2(a, b);
+        if (threadIdx.x == 0) coef[n * g.G + group] = make_float2(a, b);
         return;
     }
     const unsigned c = blockIdx.x - groups;
@@ -454,7 +459,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_apply_kernel(const 
     constexpr int U = unroll_bwd<V>();
     const unsigned block = backwards ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
     const int s = block % g.S, slab = block / g.S % g.nslab;
-    const int64_t n = block / g.S / g.nslab;
+    const int64_t n = g.n0 + block / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
@@ -557,7 +562,7 @@ __global__ __launch_bounds__((small_bound<V, K, false>())) void norm_small_kerne
 {
     extern __shared__ double small_buf[];              // blockDim * V slots, then two values a group
     double* buf = small_buf;
-    const int64_t n = blockIdx.x / (unsigned)g.nslab;
+    const int64_t n = g.n0 + blockIdx.x / (unsigned)g.nslab;
     const int c0 = (int)(blockIdx.x % (unsigned)g.nslab) * g.Cs, cs = min(g.Cs, g.C - c0), cols = cs / V;
     const int R = blockDim.x / cols, T = R * cols, t = threadIdx.x, P = (int)g.P;
     double* group_mean = buf + blockDim.x * V;
@@ -621,7 +626,7 @@ __global__ __launch_bounds__((small_bound<V, K, true>())) void norm_small_bwd_ke
 {
     extern __shared__ double small_buf[];
     float* buf = (float*)small_buf;
-    const int64_t n = blockIdx.x / (unsigned)g.nslab;
+    const int64_t n = g.n0 + blockIdx.x / (unsigned)g.nslab;
     const int c0 = (int)(blockIdx.x % (unsigned)g.nslab) * g.Cs, cs = min(g.Cs, g.C - c0), cols = cs / V;
     const int R = blockDim.x / cols, T = R * cols, t = threadIdx.x, P = (int)g.P;
     float* s1 = buf + blockDim.x * V;
@@ -733,6 +738,17 @@ static SmallGeom small_geom(const NormGeom& g, int V, int bytes, bool backward)
     return q;
 }
 
+// Calls launch(geometry of some samples, its workgroups) until all samples are through: a launch takes less than 2^32 threads.
+template <typename F> static void by_samples(NormGeom g, int64_t blocks, unsigned threads, F launch)
+{
+    const int64_t most = ((1LL << 32) - 1) / threads / blocks;          // at least 3: `blocks` workgroups a sample are 2^20 at most
+    for (int64_t n = 0; n < g.N; n += most) {
+        g.n0 = (int)n;
+        g.n1 = (int)(g.N - n < most ? g.N - n : most);
+        launch(g, (unsigned)(g.n1 * blocks));
+    }
+}
+
 size_t group_norm_workspace_bytes(int N, int C, int G) { return (size_t)(norm_part_bytes(N, C) + (int64_t)N * G * (int64_t)sizeof(float2)); }
 
 // threads of a joining workgroup over `count` partial sums: whole waves, four values a thread while there are no more than 1024
@@ -743,61 +759,86 @@ static unsigned join_threads(int64_t count)
 }
 
 template <typename T_, int V, int ACT>
-static void small_fwd(const void* x, NormGeom g, const SmallGeom& q, const float* w, const float* b, double eps, void* y, double2* stats, hipStream_t s)
+static void fwd_launch(const void* x_, const NormGeom& g, const float* w, const float* b, double eps, void* y_, double2* stats, double2* part, hipStream_t s)
 {
-    g.Cs = q.Cs; g.nslab = q.nslab;
-    const unsigned blocks = (unsigned)((int64_t)g.N * q.nslab), lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(double));
-    if (q.K == 2) norm_small_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
-    else if (q.K == 4) norm_small_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
-    else if (q.K == 8) norm_small_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
-    else norm_small_kernel<T_, V, ACT, 16><<<blocks, q.T, lds, s>>>((const T_*)x, g, w, b, eps, (T_*)y, stats);
-}
-
-template <typename T_, int V>
-static void fwd_launch(const void* x, const NormGeom& g, const float* w, const float* b, double eps, int act, void* y, double2* stats, double2* part, hipStream_t s)
-{
+    const T_* x = (const T_*)x_;
+    T_* y = (T_*)y_;
     const SmallGeom q = small_geom(g, V, sizeof(T_), false);
     if (q.K) {
-        if (act == RAFTCORR_ACT_RELU) small_fwd<T_, V, RAFTCORR_ACT_RELU>(x, g, q, w, b, eps, y, stats, s);
-        else if (act == RAFTCORR_ACT_SILU) small_fwd<T_, V, RAFTCORR_ACT_SILU>(x, g, q, w, b, eps, y, stats, s);
-        else small_fwd<T_, V, RAFTCORR_ACT_NONE>(x, g, q, w, b, eps, y, stats, s);
+        NormGeom h = g;
+        h.Cs = q.Cs; h.nslab = q.nslab;
+        const unsigned lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(double));
+        by_samples(h, q.nslab, q.T, [&](const NormGeom& h, unsigned blocks) {
+            if (q.K == 2) norm_small_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
+            else if (q.K == 4) norm_small_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
+            else if (q.K == 8) norm_small_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
+            else norm_small_kernel<T_, V, ACT, 16><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
+        });
         return;
     }
-    const unsigned blocks = (unsigned)((int64_t)g.N * g.nslab * g.S), joins = (unsigned)((int64_t)g.N * g.G);
-    norm_stats_kernel<T_, V><<<blocks, kThreads, 0, s>>>((const T_*)x, g, part);
-    norm_join_kernel<<<joins, join_threads((int64_t)g.S * g.D), 0, s>>>(part, g, eps, stats);
-    if (act == RAFTCORR_ACT_RELU) norm_apply_kernel<T_, V, RAFTCORR_ACT_RELU><<<blocks, kThreads, 0, s>>>((const T_*)x, g, stats, w, b, (T_*)y);
-    else if (act == RAFTCORR_ACT_SILU) norm_apply_kernel<T_, V, RAFTCORR_ACT_SILU><<<blocks, kThreads, 0, s>>>((const T_*)x, g, stats, w, b, (T_*)y);
-    else norm_apply_kernel<T_, V, RAFTCORR_ACT_NONE><<<blocks, kThreads, 0, s>>>((const T_*)x, g, stats, w, b, (T_*)y);
+    const unsigned threads = join_threads((int64_t)g.S * g.D);
+    by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) { norm_stats_kernel<T_, V><<<blocks, kThreads, 0, s>>>(x, h, part); });
+    by_samples(g, g.G, threads, [&](const NormGeom& h, unsigned blocks) { norm_join_kernel<<<blocks, threads, 0, s>>>(part, h, eps, stats); });
+    by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
+        norm_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>(x, h, stats, w, b, y);
+    });
 }
 
 template <typename T_, int V, int ACT>
-static void bwd_launch(const void* x, const void* dy, const NormGeom& g, const float* w, const float* b, const double2* stats, void* dx,
+static void bwd_launch(const void* x_, const void* dy_, const NormGeom& g, const float* w, const float* b, const double2* stats, void* dx_,
                        float* dw, float* db, float2* part, float2* coef, hipStream_t s)
 {
+    const T_ *x = (const T_*)x_, *dy = (const T_*)dy_;
+    T_* dx = (T_*)dx_;
     const SmallGeom q = small_geom(g, V, sizeof(T_), true);
     if (q.K) {
         NormGeom h = g;
         h.Cs = q.Cs; h.nslab = q.nslab; h.S = 1; h.rows = g.P;
         const bool join = (dw || db) && g.N > 1;
-        const unsigned blocks = (unsigned)((int64_t)g.N * q.nslab), lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(float));
+        const unsigned lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(float));
         float2* sums = join ? part : nullptr;
         float *dw1 = join ? nullptr : dw, *db1 = join ? nullptr : db;
-        if (q.K == 2) norm_small_bwd_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>((const T_*)x, (const T_*)dy, h, stats, w, b, (T_*)dx, sums, dw1, db1);
-        else if (q.K == 4) norm_small_bwd_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>((const T_*)x, (const T_*)dy, h, stats, w, b, (T_*)dx, sums, dw1, db1);
-        else norm_small_bwd_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>((const T_*)x, (const T_*)dy, h, stats, w, b, (T_*)dx, sums, dw1, db1);
-        h.G = 0;                                                       // the channels' sums alone
+        by_samples(h, q.nslab, q.T, [&](const NormGeom& h, unsigned blocks) {
+            if (q.K == 2) norm_small_bwd_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
+            else if (q.K == 4) norm_small_bwd_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
+            else norm_small_bwd_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
+        });
+        h.n1 = 0;                                                      // the channels' sums alone
         if (join) norm_bwd_join_kernel<<<g.C, join_threads(g.N), 0, s>>>(part, h, w, coef, dw, db);
         return;
     }
-    const unsigned blocks = (unsigned)((int64_t)g.N * g.nslab * g.S);
-    const unsigned joins = (unsigned)((int64_t)g.N * g.G + (dw || db ? g.C : 0));
+    // the groups' sums, and in the last launch the channels'
     const int64_t most = (int64_t)g.S * g.D > (dw || db ? (int64_t)g.S * g.N : 0) ? (int64_t)g.S * g.D : (int64_t)g.S * g.N;
-    norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>((const T_*)x, (const T_*)dy, g, stats, w, b, part);
-    norm_bwd_join_kernel<<<joins, join_threads(most), 0, s>>>(part, g, w, coef, dw, db);
-    const int backwards = 2 * g.N * g.P * g.C * (int64_t)sizeof(T_) > 256 << 20;
-    if (dx) norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>((const T_*)x, (const T_*)dy, g, stats, w, b, coef, (T_*)dx,
-                                                                               backwards);
+    const unsigned threads = join_threads(most);
+    by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
+        norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>(x, dy, h, stats, w, b, part);
+    });
+    by_samples(g, g.G, threads, [&](const NormGeom& h, unsigned blocks) {
+        const bool last = h.n0 + h.n1 == g.N && (dw || db);
+        norm_bwd_join_kernel<<<blocks + (last ? g.C : 0), threads, 0, s>>>(part, h, w, coef, dw, db);
+    });
+    const int backwards = (int64_t)g.N * g.P * g.C * (int64_t)sizeof(T_) > 128 << 20;         // beyond the last-level cache: what was read last first
+    if (dx) by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
+        norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>(x, dy, h, stats, w, b, coef, dx, backwards);
+    });
+}
+
+// f(a value of the element type, the vector's length, the activation) for the run-time ones
+template <typename F> static void dispatch(int dtype, int V, int act, F f)
+{
+    auto with_act = [&](auto t, auto v) {
+        if (act == RAFTCORR_ACT_RELU) f(t, v, std::integral_constant<int, RAFTCORR_ACT_RELU>());
+        else if (act == RAFTCORR_ACT_SILU) f(t, v, std::integral_constant<int, RAFTCORR_ACT_SILU>());
+        else f(t, v, std::integral_constant<int, RAFTCORR_ACT_NONE>());
+    };
+    auto with_vector = [&](auto t) {
+        constexpr int full = 16 / (int)sizeof(t);
+        if (V == full) with_act(t, std::integral_constant<int, full>());
+        else with_act(t, std::integral_constant<int, 1>());
+    };
+    if (dtype == RAFTCORR_DTYPE_FP32) with_vector(float());
+    else if (dtype == RAFTCORR_DTYPE_FP16) with_vector(_Float16());
+    else with_vector(__bf16());
 }
 
 int launch_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dtype, int N, int64_t P, int C, int G, const float* w,
@@ -808,23 +849,10 @@ int launch_group_norm_fwd(const void* x, int64_t x_batch, int64_t x_row, int dty
     if (V > 1 && small_geom(g, 1, dtype == RAFTCORR_DTYPE_FP32 ? 4 : 2, false).K && C % V) V = 1;
     double2* part = (double2*)workspace;
     double2* st = (double2*)stats;
-    if (dtype == RAFTCORR_DTYPE_FP32) {
-        if (V == 4) fwd_launch<float, 4>(x, g, w, b, eps, act, y, st, part, s); else fwd_launch<float, 1>(x, g, w, b, eps, act, y, st, part, s);
-    } else if (dtype == RAFTCORR_DTYPE_FP16) {
-        if (V == 8) fwd_launch<_Float16, 8>(x, g, w, b, eps, act, y, st, part, s); else fwd_launch<_Float16, 1>(x, g, w, b, eps, act, y, st, part, s);
-    } else {
-        if (V == 8) fwd_launch<__bf16, 8>(x, g, w, b, eps, act, y, st, part, s); else fwd_launch<__bf16, 1>(x, g, w, b, eps, act, y, st, part, s);
-    }
+    dispatch(dtype, V, act, [&](auto t, auto v, auto a) {
+        fwd_launch<decltype(t), decltype(v)::value, decltype(a)::value>(x, g, w, b, eps, y, st, part, s);
+    });
     return check_launch("group_norm_fwd");
-}
-
-template <typename T_, int V>
-static void bwd_by_act(int act, const void* x, const void* dy, const NormGeom& g, const float* w, const float* b, const double2* stats, void* dx,
-                       float* dw, float* db, float2* part, float2* coef, hipStream_t s)
-{
-    if (act == RAFTCORR_ACT_RELU) bwd_launch<T_, V, RAFTCORR_ACT_RELU>(x, dy, g, w, b, stats, dx, dw, db, part, coef, s);
-    else if (act == RAFTCORR_ACT_SILU) bwd_launch<T_, V, RAFTCORR_ACT_SILU>(x, dy, g, w, b, stats, dx, dw, db, part, coef, s);
-    else bwd_launch<T_, V, RAFTCORR_ACT_NONE>(x, dy, g, w, b, stats, dx, dw, db, part, coef, s);
 }
 
 int launch_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const void* dy, int64_t d_batch, int64_t d_row, int dtype, int N,
@@ -837,16 +865,9 @@ int launch_group_norm_bwd(const void* x, int64_t x_batch, int64_t x_row, const v
     float2* part = (float2*)workspace;
     float2* coef = (float2*)((char*)workspace + norm_part_bytes(N, C));
     const double2* st = (const double2*)stats;
-    if (dtype == RAFTCORR_DTYPE_FP32) {
-        if (V == 4) bwd_by_act<float, 4>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
-        else bwd_by_act<float, 1>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
-    } else if (dtype == RAFTCORR_DTYPE_FP16) {
-        if (V == 8) bwd_by_act<_Float16, 8>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
-        else bwd_by_act<_Float16, 1>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
-    } else {
-        if (V == 8) bwd_by_act<__bf16, 8>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
-        else bwd_by_act<__bf16, 1>(act, x, dy, g, w, b, st, dx, dw, db, part, coef, s);
-    }
+    dispatch(dtype, V, act, [&](auto t, auto v, auto a) {
+        bwd_launch<decltype(t), decltype(v)::value, decltype(a)::value>(x, dy, g, w, b, st, dx, dw, db, part, coef, s);
+    });
     return check_launch("group_norm_bwd");
 }
 

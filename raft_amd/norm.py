@@ -18,7 +18,9 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none
     The result has x's type and lies channels-last (for four dimensions: torch.channels_last).  x is read in place where its
     channels are neighbours and its positions evenly spaced (channels-last tensors, their channel or batch slices); any other
     layout is copied first, and so is the gradient that comes back.  Statistics are summed in float64,
-    gradients in float32, whatever x's type.  An empty x gives an empty result."""
+    gradients in float32, whatever x's type.  An empty x gives an empty result.
+
+    Forward and backward passes can be captured into a HIP graph; a leaf of which an eager graph is still alive is refused there."""
     act = _lib.ACTIVATIONS.get("none" if activation is None else activation)
     if act is None:
         raise RuntimeError(f"activation must be one of {sorted(_lib.ACTIVATIONS)}, got {activation!r}")

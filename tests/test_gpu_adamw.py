@@ -403,6 +403,15 @@ def test_refusals(dev):
     assert opt.step(lambda: torch.tensor(3.0)) == 3.0
     with pytest.raises(ValueError, match="lr"):
         AdamW([p], lr=torch.zeros(2))
+    whole = torch.zeros(40, device=dev)
+    for pair in ((whole[:30], whole[20:]), (whole[3:8], whole)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            AdamW([torch.nn.Parameter(t) for t in pair])._ready()
+    with pytest.warns(UserWarning, match="duplicate"):
+        twice = AdamW([p, p])
+    with pytest.raises(RuntimeError, match="share memory"):
+        twice._ready()
+    AdamW([torch.nn.Parameter(whole[:30]), torch.nn.Parameter(whole[30:])])._ready()
     with pytest.raises(RuntimeError, match="decoded"):
         AdamW([p], state_bits=8).packed_moments(torch.float64)
 

@@ -310,3 +310,67 @@ def test_offsets_beyond_32_bits(dev):
         col = x[n, channel].double()
         want = (x[n, channel, at[1], at[2]].double() - col.mean()) / (col.var(unbiased=False) + 1e-5).sqrt()
         assert abs(y[n, channel, at[1], at[2]].double() - want) <= 2.0 ** -11 * abs(want) + 1e-4
+
+
+def test_more_samples_than_a_launch_takes(dev):
+    """2^24 + 100 samples of one row: a workgroup each would be 2^32 threads and more.  The channels' sums run over all samples: 64 u of
+    the sum of sizes, and x's type is exact enough for d(y) = 1 to make d(bias) a count."""
+    from raft_amd import group_norm
+    N, C = (1 << 24) + 100, 8
+    x = torch.empty(N, C, dtype=torch.float16, device=dev).normal_().requires_grad_(True)
+    w, b = torch.ones(C, device=dev, requires_grad=True), torch.zeros(C, device=dev, requires_grad=True)
+    y = group_norm(x, 2, w, b, activation="relu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    for at in (slice(0, 1000), slice((1 << 24) - 500, (1 << 24) + 100)):
+        want = formula(x[at].detach(), w, b, 2, 1e-5, "relu", torch.ones_like(x[at]))
+        near("y", y[at], want[0])
+        near("dx", dx[at], want[1])
+    passed, xh = torch.zeros(C, dtype=torch.float64, device=dev), torch.zeros(C, dtype=torch.float64, device=dev)
+    sizes = xh.clone()
+    for part in x.detach().split(1 << 21):
+        d = part.double().view(-1, 2, 4)
+        d = d - d.mean(2, keepdim=True)
+        z = (d / ((d * d).mean(2, keepdim=True) + 1e-5).sqrt()).view(-1, C)
+        passed += (z > 0).sum(0)
+        xh += (z * (z > 0)).sum(0)
+        sizes += (z * (z > 0)).abs().sum(0)
+    assert ((db.double() - passed).abs() <= U * passed).all()
+    assert ((dw.double() - xh).abs() <= U * sizes).all()
+
+
+def test_capture_with_a_live_eager_graph_is_refused(dev):
+    from raft_amd import group_norm
+    x = torch.randn(2, 8, 6, 7, device=dev).contiguous(memory_format=torch.channels_last).requires_grad_(True)
+    dy = torch.ones_like(x)
+    eager = group_norm(x, 2)
+    with pytest.raises(RuntimeError, match="eager graph of x is alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            group_norm(x, 2)
+    want, = torch.autograd.grad(eager, x, dy)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(group_norm(x, 2), x, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_no_second_derivative(dev):
+    from raft_amd import group_norm
+    x = torch.randn(2, 8, 6, 7, device=dev, requires_grad=True)
+    dx, = torch.autograd.grad(group_norm(x, 2).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dx.sum().backward()
+
+
+def test_refusals(dev):
+    from raft_amd import group_norm
+    x = torch.randn(2, 8, 6, 7, device=dev)
+    for args, words in (((x, 3), "does not divide"), ((x, 0), "does not divide"), ((x.double(), 2), "float32, float16 or bfloat16"), ((x[0, 0, 0], 1), "shape"),
+                        ((x, 2, torch.ones(7, device=dev)), "weight must be"), ((x, 2, None, torch.ones(8)), "bias is on cpu"),
+                        ((x, 2, torch.ones(8, device=dev).int()), "weight must be"), ((x, 2, None, None, -1.0), "eps")):
+        with pytest.raises(RuntimeError, match=words):
+            group_norm(*args)
+    with pytest.raises(RuntimeError, match="activation"):
+        group_norm(x, 2, activation="gelu")

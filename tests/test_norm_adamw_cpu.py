@@ -86,7 +86,7 @@ def test_c_abi_refuses_without_touching_the_gpu():
     for bad in (dict(x=None), dict(y=None), dict(stats=None), dict(work=None), dict(bytes_=ws - 1), dict(row=7), dict(dtype=3), dict(N=0), dict(P=0),
                 dict(C=0), dict(G=3), dict(G=0), dict(act=3), dict(eps=-1.0), dict(eps=float("nan"))):
         assert fwd(**bad) == -1, bad
-    assert lib.raftcorr_group_norm_fwd(16, 0, 8, 0, 1 << 30, 4, 8, 8, None, None, 1e-5, 0, 16, 16, 16, 1 << 62, None) == -2
+    assert lib.raftcorr_group_norm_fwd(16, 0, 1 << 21, 0, 1, 4, 1 << 21, 8, None, None, 1e-5, 0, 16, 16, 16, 1 << 62, None) == -2
     assert lib.raftcorr_group_norm_bwd(16, 0, 8, 16, 0, 7, 0, 2, 4, 8, 2, None, None, 0, 16, 16, None, None, 16, ws, None) == -1
     assert b"overlap" in lib.raftcorr_last_error()
     ptr, n = (ctypes.c_void_p * 1)(16), (ctypes.c_int64 * 1)(5)
