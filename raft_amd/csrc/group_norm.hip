@@ -36,8 +36,9 @@ enum {
     kWaves = 4,                  // workgroups a CU (registers: 128 a thread)
     kUnroll = 4,                 // vectors of x that a thread has on their way at once, forward
     kMostRanges = 1024,          // workgroups of a pass over everything ...
-    kFewRanges = 512,            // ... and while a range stays below kRangeBytes: each workgroup costs a launch, its coefficients and a join
-    kRangeBytes = 256 << 10,     // (2 x 64 x 220 x 512 float32, forward: 512 take 34 us, 1024 36; 12 x 64 x 200 x 360: 117 and 109)
+    kFewRanges = 768,            // ... and while these leave a range below kRangeBytes: each workgroup costs a launch, its coefficients and a join
+    kRangeBytes = 192 << 10,     // (forward + backward in us; 12 x 128 x 50 x 90 float16: 17.2 + 22.9, with 1024 18.7 + 24.1;
+                                 // 12 x 64 x 200 x 360 float32: with 512 117 + 199, with 1024 109 + 184)
 };
 
 // the same backward, of x and of dy each
@@ -71,22 +72,17 @@ template <int V> __device__ __forceinline__ void slab_of(const NormGeom& g, int 
     if (cs != g.Cs) { const int cols = cs / V; R = kThreads / cols; T = R * cols; }   // last slab: V divides its width (or V == 1)
 }
 
-// Row lane, channel and group of each of a thread's V slots (slot j: value t * V + j of a round), by one division each and counting.
+// Row lane and column of each of a thread's V slots (slot j: value t * V + j of a round), by one division and counting.
 template <int V> struct Slots {
-    int lane[V], c[V], group[V];
-    int col;                                         // first slot's column in the slab
-    __device__ __forceinline__ Slots(const NormGeom& g, int t, int c0, int cs)
+    int lane[V], col[V];
+    __device__ __forceinline__ Slots(int t, int cs)
     {
         const unsigned f = (unsigned)t * V;
         int l = (int)(f / (unsigned)cs), k = (int)(f % (unsigned)cs);
-        col = k;
-        int p = (int)((unsigned)(c0 + k) / (unsigned)g.D), rest = (c0 + k) - p * g.D;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            lane[j] = l; c[j] = c0 + k; group[j] = p;
-            ++k; ++rest;
-            if (rest == g.D) { rest = 0; ++p; }
-            if (k == cs) { k = 0; ++l; rest = 0; p = 0; }            // only where the slab is the whole row: from channel 0 again
+            lane[j] = l; col[j] = k;
+            if (++k == cs) { k = 0; ++l; }                          // only where the slab is the whole row
         }
     }
 };
@@ -127,7 +123,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* 
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
     double sum[V] = {}, squares[V] = {};
     if (t < T) {
-        const Slots<V> q(g, t, c0, cs);
+        const Slots<V> q(t, cs);
         const int (&lane)[V] = q.lane;
         auto add = [&](T_ e, int j) {
             const double d = (double)to_float(e);
@@ -136,7 +132,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* 
         };
         const int64_t step = (int64_t)R * g.x_row;
         int64_t r = s * g.rows;
-        const T_* p = x + n * g.x_batch + (r + lane[0]) * g.x_row + c0 + q.col;
+        const T_* p = x + n * g.x_batch + (r + lane[0]) * g.x_row + c0 + q.col[0];
         for (; r + (int64_t)U * R <= r1; r += U * R) {
             Vec<T_, V> v[U];
 #pragma unroll
@@ -234,6 +230,18 @@ template <int ACT> __device__ __forceinline__ float slope(float z)
     return 1.f;
 }
 
+// What the slots need of their channels is worked out once a channel and handed to them through shared memory: with loads by every
+// slot for itself 12 x 128 x 50 x 90 float16 takes 20.1 us forward and 28.1 backward, this way 17.2 and 22.9.
+// [mean][rstd w][b], each cs floats
+__device__ __forceinline__ void stage_forward(float* lds, int c, int cs, double2 st, const float* weight, const float* bias, int channel)
+{
+    lds[c] = (float)st.x;
+    lds[cs + c] = (float)st.y * (weight ? weight[channel] : 1.f);
+    lds[2 * cs + c] = bias ? bias[channel] : 0.f;
+}
+
+extern __shared__ float staged[];
+
 template <typename T_, int V, int ACT>
 __global__ __launch_bounds__(kThreads, kWaves) void norm_apply_kernel(const T_* __restrict__ x, NormGeom g, const double2* __restrict__ stats,
                                                               const float* __restrict__ weight, const float* __restrict__ bias,
@@ -245,22 +253,22 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_apply_kernel(const T_* 
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
+    for (int c = t; c < cs; c += kThreads) stage_forward(staged, c, cs, stats[n * g.G + (c0 + c) / g.D], weight, bias, c0 + c);
+    __syncthreads();
     if (t >= T) return;
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
     float mean[V], a[V], b[V];
-    const Slots<V> q(g, t, c0, cs);
+    const Slots<V> q(t, cs);
     const int (&lane)[V] = q.lane;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = q.c[j];
-        const double2 st = stats[n * g.G + q.group[j]];
-        mean[j] = (float)st.x;
-        a[j] = (float)st.y * (weight ? weight[c] : 1.f);
-        b[j] = bias ? bias[c] : 0.f;
+        mean[j] = staged[q.col[j]];
+        a[j] = staged[cs + q.col[j]];
+        b[j] = staged[2 * cs + q.col[j]];
     }
     const int64_t step = (int64_t)R * g.x_row, ystep = (int64_t)R * g.C;
-    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col;
-    T_* o = y + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + q.col;
+    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col[0];
+    T_* o = y + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + q.col[0];
     int64_t r = s * g.rows;
     for (; r + (int64_t)U * R <= r1; r += U * R) {
         Vec<T_, V> v[U];
@@ -297,11 +305,13 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_apply_kernel(const T_* 
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 
-// What a slot needs of its channel.  ReLU passes a gradient where z = (x - mean) rstd w + b > 0, that is where x is above (for w < 0:
+// What a channel's slots need.  ReLU passes a gradient where z = (x - mean) rstd w + b > 0, that is where x is above (for w < 0:
 // below) the point mean - b / (rstd w).  That point is computed in 64 bits and rounded down to a float32 `edge`, and x, with its
 // sign turned for w < 0, is compared with it: the right side for every x, one operation instead of two.  With z in float32 one in
 // some 10^8 values would land on the wrong side, and its whole gradient with it.
-struct NormCoef { float mean, rstd, w, b, turn, edge; };
+//   g = dy act'(z):  ReLU: dy where x * k0 > k1 (turn, edge);  SiLU: z = (x - mean) * k0 + k1 (rstd w, b)
+//   dx = g * a - b - (x - mean) * c,  a = rstd w, b = rstd s1, c = rstd^2 s2
+enum { kMean, kSlope0, kSlope1, kSums, kA = kSums, kB, kC, kFields };          // rows of `staged`; the sums need the first three
 
 __device__ __forceinline__ float round_down(double d)
 {
@@ -312,27 +322,45 @@ __device__ __forceinline__ float round_down(double d)
 }
 
 template <int ACT>
-__device__ __forceinline__ NormCoef coef_of(double2 st, const float* weight, const float* bias, int c)
+__device__ __forceinline__ void stage_backward(float* lds, int c, int cs, double2 st, const float* weight, const float* bias, int channel)
 {
-    NormCoef k{(float)st.x, (float)st.y, weight ? weight[c] : 1.f, bias ? bias[c] : 0.f, 1.f, 0.f};
+    const float w = weight ? weight[channel] : 1.f, b = bias ? bias[channel] : 0.f;
+    lds[kMean * cs + c] = (float)st.x;
     if (ACT == RAFTCORR_ACT_RELU) {
-        k.turn = k.w < 0.f ? -1.f : 1.f;
-        const double scale = (double)k.w * st.y;
-        double r = __builtin_amdgcn_rcp(scale);             // two Newton steps: 64 bits (half the instructions of a division)
-        r = fma(r, fma(-scale, r, 1.0), r);
-        r = fma(r, fma(-scale, r, 1.0), r);
-        const double at = st.x - (k.b != 0.f ? (double)k.b * r : 0.0);
-        k.edge = k.w == 0.f ? (k.b > 0.f ? -__builtin_inff() : __builtin_inff()) : round_down(k.turn * at);
+        const float turn = w < 0.f ? -1.f : 1.f;
+        const double at = st.x - (b != 0.f ? (double)b / ((double)w * st.y) : 0.0);
+        lds[kSlope0 * cs + c] = turn;
+        lds[kSlope1 * cs + c] = w == 0.f ? (b > 0.f ? -__builtin_inff() : __builtin_inff()) : round_down(turn * at);
+    } else if (ACT == RAFTCORR_ACT_SILU) {
+        lds[kSlope0 * cs + c] = (float)st.y * w;
+        lds[kSlope1 * cs + c] = b;
     }
-    return k;
 }
 
-// g = dy * act'(z)
-template <int ACT> __device__ __forceinline__ float through(const NormCoef& k, float x, float xh, float dy)
+__device__ __forceinline__ void stage_gradient(float* lds, int c, int cs, double2 st, const float* weight, float s1, float s2, int channel)
 {
-    if (ACT == RAFTCORR_ACT_RELU) return x * k.turn > k.edge ? dy : 0.f;
-    return dy * slope<ACT>(xh * k.w + k.b);
+    const float rstd = (float)st.y;
+    lds[kA * cs + c] = rstd * (weight ? weight[channel] : 1.f);
+    lds[kB * cs + c] = rstd * s1;
+    lds[kC * cs + c] = rstd * rstd * s2;
 }
+
+// a slot's share of them
+template <int ACT> struct NormCoef {
+    float mean, k0, k1;
+    __device__ __forceinline__ void take(const float* lds, int col, int cs)
+    {
+        mean = lds[kMean * cs + col];
+        k0 = ACT == RAFTCORR_ACT_NONE ? 0.f : lds[kSlope0 * cs + col];
+        k1 = ACT == RAFTCORR_ACT_NONE ? 0.f : lds[kSlope1 * cs + col];
+    }
+    // g = dy * act'(z), d = x - mean
+    __device__ __forceinline__ float through(float x, float d, float dy) const
+    {
+        if (ACT == RAFTCORR_ACT_RELU) return x * k0 > k1 ? dy : 0.f;
+        return dy * slope<ACT>(d * k0 + k1);
+    }
+};
 
 // sum of g and of g * xh of each channel over one row range -> part[n][s][c]
 template <typename T_, int V, int ACT>
@@ -348,22 +376,23 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_sums_kernel(const T
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
-    float sum[V] = {}, dot[V] = {};
+    for (int c = t; c < cs; c += kThreads) stage_backward<ACT>(staged, c, cs, stats[n * g.G + (c0 + c) / g.D], weight, bias, c0 + c);
+    __syncthreads();
+    float sum[V] = {}, dot[V] = {};                          // of g and of g * (x - mean)
     if (t < T) {
-        NormCoef k[V];
-        const Slots<V> q(g, t, c0, cs);
+        NormCoef<ACT> k[V];
+        const Slots<V> q(t, cs);
         const int (&lane)[V] = q.lane;
 #pragma unroll
-        for (int j = 0; j < V; ++j) k[j] = coef_of<ACT>(stats[n * g.G + q.group[j]], weight, bias, q.c[j]);
+        for (int j = 0; j < V; ++j) k[j].take(staged, q.col[j], cs);
         auto add = [&](float xv, float dv, int j, float& a, float& b) {
-            const float xh = (xv - k[j].mean) * k[j].rstd;
-            const float e = through<ACT>(k[j], xv, xh, dv);
+            const float d = xv - k[j].mean, e = k[j].through(xv, d, dv);
             a += e;
-            b += e * xh;
+            b += e * d;
         };
         const int64_t step = (int64_t)R * g.x_row, dstep = (int64_t)R * g.d_row;
-        const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col;
-        const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + q.col;
+        const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col[0];
+        const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + q.col[0];
         int64_t r = s * g.rows;
         for (; r + (int64_t)U * R <= r1; r += U * R) {
             Vec<T_, V> v[U], w[U];
@@ -405,7 +434,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_sums_kernel(const T
     reduce_columns<V>(sum, buf, T, R, cs);
     for (int c = t; c < cs; c += kThreads) out[c].x = buf[c];
     reduce_columns<V>(dot, buf, T, R, cs);
-    for (int c = t; c < cs; c += kThreads) out[c].y = buf[c];
+    for (int c = t; c < cs; c += kThreads) out[c].y = buf[c] * (float)stats[n * g.G + (c0 + c) / g.D].y;
 }
 
 // part -> (s1, s2) of each (n, group) and, in further workgroups with dweight / dbias, a channel's sums over all samples
@@ -463,26 +492,33 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_apply_kernel(const 
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
+    for (int c = t; c < cs; c += kThreads) {
+        const int64_t group = n * g.G + (c0 + c) / g.D;
+        stage_backward<ACT>(staged, c, cs, stats[group], weight, bias, c0 + c);
+        stage_gradient(staged, c, cs, stats[group], weight, coef[group].x, coef[group].y, c0 + c);
+    }
+    __syncthreads();
     if (t >= T) return;
     const int64_t r1 = min(g.P, (s + 1) * g.rows);
-    NormCoef k[V];
-    float2 m[V];
-    const Slots<V> q(g, t, c0, cs);
+    NormCoef<ACT> k[V];
+    float ka[V], kb[V], kc[V];
+    const Slots<V> q(t, cs);
     const int (&lane)[V] = q.lane;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        k[j] = coef_of<ACT>(stats[n * g.G + q.group[j]], weight, bias, q.c[j]);
-        m[j] = coef[n * g.G + q.group[j]];
+        k[j].take(staged, q.col[j], cs);
+        ka[j] = staged[kA * cs + q.col[j]];
+        kb[j] = staged[kB * cs + q.col[j]];
+        kc[j] = staged[kC * cs + q.col[j]];
     }
     auto grad = [&](float xv, float dv, int j) {
-        const float xh = (xv - k[j].mean) * k[j].rstd;
-        const float e = through<ACT>(k[j], xv, xh, dv);
-        return k[j].rstd * (e * k[j].w - m[j].x - xh * m[j].y);
+        const float d = xv - k[j].mean;
+        return k[j].through(xv, d, dv) * ka[j] - kb[j] - d * kc[j];
     };
     const int64_t step = (int64_t)R * g.x_row, dstep = (int64_t)R * g.d_row, ostep = (int64_t)R * g.C;
-    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col;
-    const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + q.col;
-    T_* o = dx + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + q.col;
+    const T_* p = x + n * g.x_batch + (s * g.rows + lane[0]) * g.x_row + c0 + q.col[0];
+    const T_* d = dy + n * g.d_batch + (s * g.rows + lane[0]) * g.d_row + c0 + q.col[0];
+    T_* o = dx + (n * g.P + s * g.rows + lane[0]) * g.C + c0 + q.col[0];
     int64_t r = s * g.rows;
     for (; r + (int64_t)U * R <= r1; r += U * R) {
         Vec<T_, V> v[U], w[U];
@@ -527,7 +563,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_apply_kernel(const 
 // ---- small: one workgroup holds a slab of whole groups of one sample --------------------------------------------------------
 
 // Slab of a workgroup: whole groups, whole vectors, 32 or 64 bytes of each row at least.  T threads, K rounds.
-struct SmallGeom { int Cs, nslab, T, K; };
+struct SmallGeom { int Cs, nslab, T, K, lds; };
 
 // most threads of such a workgroup: the slots' sums take 32 KB
 template <int V> constexpr int small_threads() { return V == 8 ? 512 : 1024; }
@@ -560,7 +596,7 @@ __global__ __launch_bounds__((small_bound<V, K, false>())) void norm_small_kerne
                                                                         const float* __restrict__ bias, double eps, T_* __restrict__ y,
                                                                         double2* __restrict__ stats)
 {
-    extern __shared__ double small_buf[];              // blockDim * V slots, then two values a group
+    extern __shared__ double small_buf[];              // blockDim * V slots, two values a group, the channels' three
     double* buf = small_buf;
     const int64_t n = g.n0 + blockIdx.x / (unsigned)g.nslab;
     const int c0 = (int)(blockIdx.x % (unsigned)g.nslab) * g.Cs, cs = min(g.Cs, g.C - c0), cols = cs / V;
@@ -589,21 +625,18 @@ __global__ __launch_bounds__((small_bound<V, K, false>())) void norm_small_kerne
     reduce_columns<V>(squares, buf, T, R, cs);
     small_groups(buf, nullptr, 1.0, group_rstd, cs, g.D);
     const double inv = 1.0 / ((double)P * (double)g.D);
-    for (int k = t; k < cs / g.D; k += blockDim.x) {
+    float* lds = (float*)(group_rstd + g.Cs / g.D);
+    for (int i = t; i < cs; i += blockDim.x) {
+        const int k = i / g.D;
         const double2 st = statistics(group_mean[k], group_rstd[k], inv, eps);
-        group_mean[k] = st.x;
-        group_rstd[k] = st.y;
-        stats[n * g.G + c0 / g.D + k] = st;
+        if (i % g.D == 0) stats[n * g.G + c0 / g.D + k] = st;
+        stage_forward(lds, i, cs, st, weight, bias, c0 + i);
     }
     __syncthreads();
     if (!work) return;
     float mean[V], a[V], b[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        mean[j] = (float)group_mean[(c + j) / g.D];
-        a[j] = (float)group_rstd[(c + j) / g.D] * (weight ? weight[c0 + c + j] : 1.f);
-        b[j] = bias ? bias[c0 + c + j] : 0.f;
-    }
+    for (int j = 0; j < V; ++j) { mean[j] = lds[c + j]; a[j] = lds[cs + c + j]; b[j] = lds[2 * cs + c + j]; }
 #pragma unroll
     for (int k = 0; k < K; ++k) keep_packed(v[k]);
     T_* o = y + (n * P + r0) * g.C + c0 + c;
@@ -642,19 +675,21 @@ __global__ __launch_bounds__((small_bound<V, K, true>())) void norm_small_bwd_ke
             v[k] = load_vec<T_, V>(p + (int64_t)k * R * g.x_row);
             d[k] = load_vec<T_, V>(q + (int64_t)k * R * g.d_row);
         }
-    NormCoef e[V];
+    float* lds = s2 + g.Cs / g.D;
+    for (int i = t; i < cs; i += blockDim.x) stage_backward<ACT>(lds, i, cs, stats[n * g.G + (c0 + i) / g.D], weight, bias, c0 + i);
+    __syncthreads();
+    NormCoef<ACT> e[V];
     float a[V], b[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         a[j] = b[j] = 0.f;
-        e[j] = work ? coef_of<ACT>(stats[n * g.G + (c0 + c + j) / g.D], weight, bias, c0 + c + j) : NormCoef{};
+        e[j].take(lds, c + j, cs);
 #pragma unroll
         for (int k = 0; k < K; ++k)
             if (work && r0 + k * R < P) {
-                const float xh = (to_float(v[k][j]) - e[j].mean) * e[j].rstd;
-                const float h = through<ACT>(e[j], to_float(v[k][j]), xh, to_float(d[k][j]));
+                const float xv = to_float(v[k][j]), m = xv - e[j].mean, h = e[j].through(xv, m, to_float(d[k][j]));
                 a[j] += h;
-                b[j] += h * xh;
+                b[j] += h * m;
             }
     }
     const float inv = 1.f / ((float)P * (float)g.D);
@@ -667,14 +702,22 @@ __global__ __launch_bounds__((small_bound<V, K, true>())) void norm_small_bwd_ke
     small_groups(buf, w, inv, s1, cs, g.D);
     reduce_columns<V>(b, buf, T, R, cs);
     for (int i = t; i < cs; i += blockDim.x) {
+        buf[i] *= (float)stats[n * g.G + (c0 + i) / g.D].y;
         if (part) part[n * g.C + c0 + i].y = buf[i];
         if (dweight) dweight[c0 + i] = buf[i];
     }
+    __syncthreads();
     if (!dx) return;
     small_groups(buf, w, inv, s2, cs, g.D);
+    for (int i = t; i < cs; i += blockDim.x)
+        stage_gradient(lds, i, cs, stats[n * g.G + (c0 + i) / g.D], weight, s1[i / g.D], s2[i / g.D], c0 + i);
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < K; ++k) { keep_packed(v[k]); keep_packed(d[k]); }
     if (!work) return;
+    float ka[V], kb[V], kc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) { ka[j] = lds[kA * cs + c + j]; kb[j] = lds[kB * cs + c + j]; kc[j] = lds[kC * cs + c + j]; }
     T_* o = dx + (n * P + r0) * g.C + c0 + c;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -682,9 +725,8 @@ __global__ __launch_bounds__((small_bound<V, K, true>())) void norm_small_bwd_ke
             Vec<T_, V> f;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (to_float(v[k][j]) - e[j].mean) * e[j].rstd;
-                const float h = through<ACT>(e[j], to_float(v[k][j]), xh, to_float(d[k][j]));
-                f[j] = from_float<T_>(e[j].rstd * (h * e[j].w - s1[(c + j) / g.D] - xh * s2[(c + j) / g.D]));
+                const float xv = to_float(v[k][j]), m = xv - e[j].mean;
+                f[j] = from_float<T_>(e[j].through(xv, m, to_float(d[k][j])) * ka[j] - kb[j] - m * kc[j]);
             }
             store_vec<T_, V>(o + (int64_t)k * R * g.C, f);
         }
@@ -733,7 +775,12 @@ static SmallGeom small_geom(const NormGeom& g, int V, int bytes, bool backward)
     for (const int T : {256, V == 8 ? small_threads<8>() : small_threads<1>()}) {
         if (cols > T) continue;
         const int64_t K = (g.P + T / cols - 1) / (T / cols);
-        if (K <= (T == 256 ? 16 : 8) / (backward ? 2 : 1)) { q.T = T; q.K = K <= 2 ? 2 : K <= 4 ? 4 : K <= 8 ? 8 : 16; return q; }
+        if (K <= (T == 256 ? 16 : 8) / (backward ? 2 : 1)) {
+            q.T = T;
+            q.lds = (T * V + 2 * (q.Cs / g.D)) * (int)(backward ? sizeof(float) : sizeof(double)) + (backward ? (int)kFields : 3) * q.Cs * (int)sizeof(float);
+            if (q.lds <= 64 << 10) q.K = K <= 2 ? 2 : K <= 4 ? 4 : K <= 8 ? 8 : 16;
+            return q;
+        }
     }
     return q;
 }
@@ -767,12 +814,11 @@ static void fwd_launch(const void* x_, const NormGeom& g, const float* w, const 
     if (q.K) {
         NormGeom h = g;
         h.Cs = q.Cs; h.nslab = q.nslab;
-        const unsigned lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(double));
         by_samples(h, q.nslab, q.T, [&](const NormGeom& h, unsigned blocks) {
-            if (q.K == 2) norm_small_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
-            else if (q.K == 4) norm_small_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
-            else if (q.K == 8) norm_small_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
-            else norm_small_kernel<T_, V, ACT, 16><<<blocks, q.T, lds, s>>>(x, h, w, b, eps, y, stats);
+            if (q.K == 2) norm_small_kernel<T_, V, ACT, 2><<<blocks, q.T, q.lds, s>>>(x, h, w, b, eps, y, stats);
+            else if (q.K == 4) norm_small_kernel<T_, V, ACT, 4><<<blocks, q.T, q.lds, s>>>(x, h, w, b, eps, y, stats);
+            else if (q.K == 8) norm_small_kernel<T_, V, ACT, 8><<<blocks, q.T, q.lds, s>>>(x, h, w, b, eps, y, stats);
+            else norm_small_kernel<T_, V, ACT, 16><<<blocks, q.T, q.lds, s>>>(x, h, w, b, eps, y, stats);
         });
         return;
     }
@@ -780,7 +826,7 @@ static void fwd_launch(const void* x_, const NormGeom& g, const float* w, const 
     by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) { norm_stats_kernel<T_, V><<<blocks, kThreads, 0, s>>>(x, h, part); });
     by_samples(g, g.G, threads, [&](const NormGeom& h, unsigned blocks) { norm_join_kernel<<<blocks, threads, 0, s>>>(part, h, eps, stats); });
     by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
-        norm_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>(x, h, stats, w, b, y);
+        norm_apply_kernel<T_, V, ACT><<<blocks, kThreads, 3 * g.Cs * sizeof(float), s>>>(x, h, stats, w, b, y);
     });
 }
 
@@ -795,13 +841,12 @@ static void bwd_launch(const void* x_, const void* dy_, const NormGeom& g, const
         NormGeom h = g;
         h.Cs = q.Cs; h.nslab = q.nslab; h.S = 1; h.rows = g.P;
         const bool join = (dw || db) && g.N > 1;
-        const unsigned lds = (unsigned)((q.T * V + 2 * (q.Cs / g.D)) * sizeof(float));
         float2* sums = join ? part : nullptr;
         float *dw1 = join ? nullptr : dw, *db1 = join ? nullptr : db;
         by_samples(h, q.nslab, q.T, [&](const NormGeom& h, unsigned blocks) {
-            if (q.K == 2) norm_small_bwd_kernel<T_, V, ACT, 2><<<blocks, q.T, lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
-            else if (q.K == 4) norm_small_bwd_kernel<T_, V, ACT, 4><<<blocks, q.T, lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
-            else norm_small_bwd_kernel<T_, V, ACT, 8><<<blocks, q.T, lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
+            if (q.K == 2) norm_small_bwd_kernel<T_, V, ACT, 2><<<blocks, q.T, q.lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
+            else if (q.K == 4) norm_small_bwd_kernel<T_, V, ACT, 4><<<blocks, q.T, q.lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
+            else norm_small_bwd_kernel<T_, V, ACT, 8><<<blocks, q.T, q.lds, s>>>(x, dy, h, stats, w, b, dx, sums, dw1, db1);
         });
         h.n1 = 0;                                                      // the channels' sums alone
         if (join) norm_bwd_join_kernel<<<g.C, join_threads(g.N), 0, s>>>(part, h, w, coef, dw, db);
@@ -811,7 +856,7 @@ static void bwd_launch(const void* x_, const void* dy_, const NormGeom& g, const
     const int64_t most = (int64_t)g.S * g.D > (dw || db ? (int64_t)g.S * g.N : 0) ? (int64_t)g.S * g.D : (int64_t)g.S * g.N;
     const unsigned threads = join_threads(most);
     by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
-        norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>(x, dy, h, stats, w, b, part);
+        norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, kSums * g.Cs * sizeof(float), s>>>(x, dy, h, stats, w, b, part);
     });
     by_samples(g, g.G, threads, [&](const NormGeom& h, unsigned blocks) {
         const bool last = h.n0 + h.n1 == g.N && (dw || db);
@@ -819,7 +864,7 @@ static void bwd_launch(const void* x_, const void* dy_, const NormGeom& g, const
     });
     const int backwards = (int64_t)g.N * g.P * g.C * (int64_t)sizeof(T_) > 128 << 20;         // beyond the last-level cache: what was read last first
     if (dx) by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
-        norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, 0, s>>>(x, dy, h, stats, w, b, coef, dx, backwards);
+        norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, kFields * g.Cs * sizeof(float), s>>>(x, dy, h, stats, w, b, coef, dx, backwards);
     });
 }
 
