@@ -53,7 +53,7 @@ static void slab_geom(NormGeom& g, int V)
     if (pattern <= kThreads) {
         g.Cs = g.C; g.nslab = 1;
         // 8 vectors of 16 bytes are a line: rounds of whole lines, or two rounds would each write a part of one
-        // (96 channels in 16 bits, 2 x 272 x 480: the writing pass takes 18 us with 240 threads, 21 with 252)
+        // (96 channels in 16 bits, 2 x 272 x 480: the writing pass takes 16 us with 240 threads, 21 with 252)
         const int lines = pattern * (8 / gcd_(pattern, 8));
         g.T = lines <= kThreads ? kThreads / lines * lines : kThreads / pattern * pattern;
     } else {
@@ -765,9 +765,9 @@ static SmallGeom small_geom(const NormGeom& g, int V, int bytes, bool backward)
     SmallGeom q{};
     const int unit = g.D / gcd_(g.D, V) * V;
     if (g.C % V) return q;
-    // 32 bytes of a row while that makes few workgroups, else 64 (lines are fetched by fewer of them); forward and backward in us,
-    // 32 | 64: 64 channels x 500 rows float32 6.0, 8.9 | 6.3, 11.0; 12 x 96 x 25 x 45 float32 10.8, 18.6 | 10.1, 15.6
-    const int least = ((int64_t)g.N * g.C * bytes < 128 * 64 ? 32 : 64) / bytes;
+    // 64 bytes of a row; forward 32 while 64 would make few workgroups (us, 32 | 64: 8 x 64 x 1000 rows float32 7.9 | 8.7,
+    // 12 x 96 x 1125 rows 11.2 | 9.7; backward 8 x 64 x 1000 rows 14.6 | 12.9)
+    const int least = (!backward && (int64_t)g.N * g.C * bytes <= 48 * 64 ? 32 : 64) / bytes;
     q.Cs = unit * ((least + unit - 1) / unit);
     if (q.Cs > g.C) q.Cs = g.C;
     q.nslab = (g.C + q.Cs - 1) / q.Cs;
