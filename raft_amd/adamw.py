@@ -21,6 +21,7 @@ class _Bucket:
     def __init__(self, params, bits, index):
         self.params, self.bits, self.index = params, bits, index
         self.device, self.dtype = params[0].device, params[0].dtype
+        self.strides = [p.stride() for p in params]
         self.glue = _lib.glue().Bucket(params)
         self.numels, self.offsets, self.total = self.glue.numels, self.glue.offsets, self.glue.total
         total = self.total
@@ -29,9 +30,14 @@ class _Bucket:
         blocks = 0 if bits == 32 else total // _lib.ADAMW_BLOCK
         self.me, self.ve = (torch.zeros(blocks, dtype=torch.uint8, device=self.device) for _ in range(2))
         self.steps = torch.zeros(len(params), dtype=torch.float32, device=self.device)
+        self.state = [self._views(i) for i in range(len(params))]        # what stands in the optimizer's state
 
-    def views(self, i):
-        """The state of parameter i as it stands in the optimizer's state."""
+    def holds(self, params):
+        """Whether the bucket is that of these parameters as they are now."""
+        return (len(params) == len(self.params) and all(p is q for p, q in zip(params, self.params)) and
+                all(p.stride() == s and p.numel() == n for p, s, n in zip(params, self.strides, self.numels)))
+
+    def _views(self, i):
         p, at = self.params[i], self.offsets[i]
         out = {"step": self.steps[i]}
         for name, flat in (("exp_avg", self.m), ("exp_avg_sq", self.v)):
@@ -64,13 +70,15 @@ class AdamW(torch.optim.Optimizer):
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"max_norm must be positive or None, got {max_norm}")
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, max_norm=max_norm, seed=int(seed))
-        self._buckets = None
+        self._buckets, self._stale, self._held = [], True, 0
         self.grad_norm = None
         super().__init__(params, defaults)
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._buckets, self.grad_norm = None, None
+        if "_buckets" not in self.__dict__:                   # unpickled or copied
+            self._buckets, self._held, self.grad_norm = [], 0, None
+        self._stale = True
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -85,17 +93,18 @@ class AdamW(torch.optim.Optimizer):
         except ValueError:
             self.param_groups.pop()
             raise
-        self._buckets = None                                 # rebuilt around the state there is
+        self._stale = True
 
     # -- state ------------------------------------------------------------------------------------------------------
 
     def _ready(self):
-        """The buckets, made on the first call and after a state was loaded or emptied."""
-        if self._buckets is not None and len(self.state) == self._held:
+        """The buckets, one list a group: made on the first call, and made to hold what `state` says after it was loaded or
+        emptied or a group was added.  Buffers of unchanged buckets stay where they are (a captured step may use them)."""
+        if not self._stale and len(self.state) >= self._held and (not self._held or self.state.get(self._first[0]) is self._first[1]):
             return self._buckets
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: take one step before a step is captured (the state is made by the first one)")
-        bits, made = self.defaults["state_bits"], []
+        bits, made, known = self.defaults["state_bits"], [], [b for buckets in self._buckets for b in buckets]
         for group in self.param_groups:
             by_kind = {}
             for p in group["params"]:
@@ -106,18 +115,25 @@ class AdamW(torch.optim.Optimizer):
                 if p.numel():
                     by_kind.setdefault((p.device, p.dtype), []).append(p)
             made.append([])
-            for params in by_kind.values():
-                made[-1].append(_Bucket(params, bits, sum(map(len, made))))
-        if _lib.glue().Bucket.overlap([p for buckets in made for b in buckets for p in b.params]):
+            for (device, dtype), params in by_kind.items():
+                index = sum(map(len, made))
+                old = [b for b in known if b.index == index and (b.device, b.dtype) == (device, dtype) and b.holds(params)]
+                made[-1].append(old[0] if old else _Bucket(params, bits, index))
+        buckets = [b for of in made for b in of]
+        if _lib.glue().Bucket.overlap([p for b in buckets for p in b.params]):
             raise RuntimeError("two parameters share memory (or one is listed twice)")
-        for buckets in made:
-            for b in buckets:
-                for i, p in enumerate(b.params):
-                    views, old = b.views(i), self.state.get(p)
+        for b in buckets:
+            for p, views in zip(b.params, b.state):
+                old = self.state.get(p)
+                if old is not views:
                     if old:
                         _adopt(views, old, bits)
+                    else:
+                        for t in views.values():
+                            t.zero_()
                     self.state[p] = views
-        self._buckets, self._held = made, len(self.state)
+        self._buckets, self._stale, self._held = made, False, sum(len(b.params) for b in buckets)
+        self._first = (buckets[0].params[0], buckets[0].state[0]) if buckets else None
         return made
 
     def load_state_dict(self, state_dict):
@@ -139,7 +155,7 @@ class AdamW(torch.optim.Optimizer):
             old = state_dict["state"].get(i)
             if old:
                 self.state[p] = {k: v.detach().clone() if torch.is_tensor(v) else v for k, v in old.items()}
-        self._buckets = None
+        self._stale = True
         if params and all(p.is_cuda for p in params):
             self._ready()
 

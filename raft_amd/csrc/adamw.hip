@@ -279,6 +279,7 @@ __global__ __launch_bounds__(kWg) void adamw_update_kernel(UpdateTable tab, Upda
             vf[j] = b2 * vv[j] + c2 * e * e;
             mv[j] = mf[j];
             vv[j] = vf[j];
+            if (j >= have) mv[j] = vv[j] = 0.f;                // padding stays zero whatever the coefficient
         }
         store_vec<float, kLane>(ms, mv);                     // a tile's state is the bucket's own: whole, padding included
         store_vec<float, kLane>(vs, vv);
@@ -298,6 +299,7 @@ __global__ __launch_bounds__(kWg) void adamw_update_kernel(UpdateTable tab, Upda
             const double e = (double)to_float(gv[j]);
             mf[j] = (float)(c1 * e + mscale * (double)code_float_signed(mw[j / 4], j % 4));
             vf[j] = (float)(c2 * e * e + vscale * (double)code_float(vw[j / 4], j % 4));
+            if (j >= have) mf[j] = vf[j] = 0.f;                         // padding stays zero whatever the coefficient
             mx = max(mx, __float_as_uint(mf[j]) & 0x7FFFFFFFu);         // as whole numbers: NaN and infinity are the largest
             vx = max(vx, __float_as_uint(vf[j]) & 0x7FFFFFFFu);
         }

@@ -78,7 +78,7 @@ def flat(t):
 def read(opt):
     """Everything the next step starts from."""
     out = []
-    for layout, b in zip(opt.packed_layout(), (b for g in opt._buckets for b in g)):
+    for layout, b in zip(opt.packed_layout(), (b for g in opt._ready() for b in g)):
         for (p, at), slot in zip(layout, range(10 ** 6)):
             n = p.numel()
             s = dict(p=flat(p), step=float(b.steps[slot]), at=at, seed=b.index * 7919)
@@ -331,6 +331,41 @@ def test_captured_step_replays(dev, bits):
         assert all(torch.equal(x, y) for x, y in zip(a.packed_moments()[0], b.packed_moments()[0]))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_buffers_stay_where_a_captured_step_expects_them(dev, bits):
+    """A state that is loaded, a group that is added, an entry that someone looks up: the captured step goes on with the state's
+    buffers, on the loaded values."""
+    from raft_amd import AdamW
+    ps = tensors(dev, [1000, 65])
+    opt = AdamW(ps, state_bits=bits, max_norm=1.0)
+    opt.step()
+    saved, then = copy.deepcopy(opt.state_dict()), [p.detach().clone() for p in ps]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    want = [p.detach().clone() for p in ps]
+    moments = [t.clone() for t in opt.packed_moments()[0]]
+    at = opt.state[ps[0]]["exp_avg"].data_ptr()
+    other = torch.zeros(3)
+    assert not opt.state[other]                                       # (a defaultdict: this makes an entry)
+    opt.add_param_group({"params": tensors(dev, [7], seed=3)})
+    opt.step()
+    del opt.state[other]
+    for p, old in zip(ps, then):
+        p.data.copy_(old)
+    rest = {k: v for k, v in opt.state_dict()["state"].items() if k > 1}
+    groups = opt.state_dict()["param_groups"]
+    opt.load_state_dict({"state": {**saved["state"], **rest}, "param_groups": groups})
+    assert opt.state[ps[0]]["exp_avg"].data_ptr() == at
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(ps, want))
+    assert all(torch.equal(x, y) for x, y in zip(opt.packed_moments()[0], moments))
+    assert float(opt.state[ps[1]]["step"]) == 2
+
+
 def test_values_that_are_not_finite(dev):
     """A NaN gradient spoils its value, with 8 bits its block's moments, and nothing else; an infinite norm clips the rest to zero."""
     from raft_amd import AdamW
@@ -351,6 +386,14 @@ def test_values_that_are_not_finite(dev):
         keep = ps[1].detach().clone()
         opt.step()
         assert torch.equal(ps[1], keep) and ps[0].isnan().sum() == 1 and math.isinf(float(opt.grad_norm))
+        ps = tensors(dev, [70, 256])                                # a coefficient of NaN spoils all values, and no gap between them
+        ps[0].grad[5] = float("nan")
+        opt = AdamW(ps, state_bits=bits, max_norm=1.0)
+        opt.step()
+        m, v = opt.packed_moments()[0]
+        assert m[:70].isnan().all() and m[512:768].isnan().all() and v[512:768].isnan().all()
+        gap = slice(128, 512) if bits == 8 else slice(70, 512)      # (blocks of 64 are spoiled as a whole)
+        assert (m[gap] == 0).all() and (v[gap] == 0).all() and (m[768:] == 0).all()
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-22, 1e-10, 1e12])
