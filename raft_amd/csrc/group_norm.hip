@@ -105,13 +105,34 @@ template <int V, typename S> __device__ __forceinline__ void reduce_columns(cons
     __syncthreads();
 }
 
+// Tensors beyond the last-level cache (256 MB) leave it with what a pass read last, and the next pass begins there (`backwards`).
+// What it could not hold anyway goes past it instead of displacing the rest: a summing pass keeps only its last kKept bytes, from
+// the workgroup `kept` on, and streams the others.  Forward of 802 MB float32 with its reading order 406 us | 420 without both;
+// backward of 221 MB twice 176 | 184, of 802 MB twice 675 | 698, of 200 MB bfloat16 twice 168 | 176.
+// Kept 128 MB: 423, 181, 691, 172; 160: 420, 178, 685, 169; 192: 411, 177, 679, 166; 240: 404, 177, 670, 170.
+constexpr int64_t kCache = 256LL << 20, kKept = 224LL << 20;
+
+template <bool ONCE, typename T_, int V>
+__device__ __forceinline__ void load_next(Vec<T_, V>& v, const T_*& p, int64_t step)
+{
+    v = ONCE ? load_vec_once<T_, V>(p) : load_vec<T_, V>(p);
+    p += step;
+}
+
+// first of a summing launch's workgroups whose rows stay in the cache; bytes: of all that the pass reads
+static unsigned kept_from(int64_t bytes, unsigned blocks)
+{
+    return bytes <= kKept ? 0 : blocks - (unsigned)((double)blocks * kKept / (double)bytes);
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------------
 
 // Sum and sum of squares of each channel over one row range -> part[n][s][c].  In 64 bits (full rate here, three operations a value):
 // no mean is large enough to cancel the squares, and the statistics are exact enough for ReLU's gradient to tell on which side of
 // zero each z lies (see NormCoef).
 template <typename T_, int V>
-__global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* __restrict__ x, NormGeom g, double2* __restrict__ part)
+__global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* __restrict__ x, NormGeom g, double2* __restrict__ part,
+                                                              unsigned kept)
 {
     constexpr int U = kUnroll;
     __shared__ double buf[kThreads * V];
@@ -135,8 +156,13 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_stats_kernel(const T_* 
         const T_* p = x + n * g.x_batch + (r + lane[0]) * g.x_row + c0 + q.col[0];
         for (; r + (int64_t)U * R <= r1; r += U * R) {
             Vec<T_, V> v[U];
+            if (blockIdx.x >= kept) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) { v[u] = load_vec<T_, V>(p); p += step; }
+                for (int u = 0; u < U; ++u) load_next<false, T_, V>(v[u], p, step);
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) load_next<true, T_, V>(v[u], p, step);
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -245,11 +271,12 @@ extern __shared__ float staged[];
 template <typename T_, int V, int ACT>
 __global__ __launch_bounds__(kThreads, kWaves) void norm_apply_kernel(const T_* __restrict__ x, NormGeom g, const double2* __restrict__ stats,
                                                               const float* __restrict__ weight, const float* __restrict__ bias,
-                                                              T_* __restrict__ y)
+                                                              T_* __restrict__ y, int backwards)
 {
     constexpr int U = kUnroll;
-    const int s = blockIdx.x % g.S, slab = blockIdx.x / g.S % g.nslab;
-    const int64_t n = g.n0 + blockIdx.x / g.S / g.nslab;
+    const unsigned block = backwards ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int s = block % g.S, slab = block / g.S % g.nslab;
+    const int64_t n = g.n0 + block / g.S / g.nslab;
     int c0, cs, T, R;
     slab_of<V>(g, slab, c0, cs, T, R);
     const int t = threadIdx.x;
@@ -366,7 +393,8 @@ template <int ACT> struct NormCoef {
 template <typename T_, int V, int ACT>
 __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_sums_kernel(const T_* __restrict__ x, const T_* __restrict__ dy, NormGeom g,
                                                                  const double2* __restrict__ stats, const float* __restrict__ weight,
-                                                                 const float* __restrict__ bias, float2* __restrict__ part)
+                                                                 const float* __restrict__ bias, float2* __restrict__ part,
+                                                                 unsigned kept)
 {
     constexpr int U = unroll_bwd<V>();
     __shared__ float buf[kThreads * V];
@@ -396,10 +424,12 @@ __global__ __launch_bounds__(kThreads, kWaves) void norm_bwd_sums_kernel(const T
         int64_t r = s * g.rows;
         for (; r + (int64_t)U * R <= r1; r += U * R) {
             Vec<T_, V> v[U], w[U];
+            if (blockIdx.x >= kept) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                v[u] = load_vec<T_, V>(p); p += step;
-                w[u] = load_vec<T_, V>(d); d += dstep;
+                for (int u = 0; u < U; ++u) { load_next<false, T_, V>(v[u], p, step); load_next<false, T_, V>(w[u], d, dstep); }
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) { load_next<true, T_, V>(v[u], p, step); load_next<true, T_, V>(w[u], d, dstep); }
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -823,10 +853,14 @@ static void fwd_launch(const void* x_, const NormGeom& g, const float* w, const 
         return;
     }
     const unsigned threads = join_threads((int64_t)g.S * g.D);
-    by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) { norm_stats_kernel<T_, V><<<blocks, kThreads, 0, s>>>(x, h, part); });
+    const int64_t bytes = (int64_t)g.N * g.P * g.C * (int64_t)sizeof(T_);
+    const int backwards = bytes > kCache;
+    by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
+        norm_stats_kernel<T_, V><<<blocks, kThreads, 0, s>>>(x, h, part, kept_from(bytes, blocks));
+    });
     by_samples(g, g.G, threads, [&](const NormGeom& h, unsigned blocks) { norm_join_kernel<<<blocks, threads, 0, s>>>(part, h, eps, stats); });
     by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
-        norm_apply_kernel<T_, V, ACT><<<blocks, kThreads, 3 * g.Cs * sizeof(float), s>>>(x, h, stats, w, b, y);
+        norm_apply_kernel<T_, V, ACT><<<blocks, kThreads, 3 * g.Cs * sizeof(float), s>>>(x, h, stats, w, b, y, backwards);
     });
 }
 
@@ -855,14 +889,15 @@ static void bwd_launch(const void* x_, const void* dy_, const NormGeom& g, const
     // the groups' sums, and in the last launch the channels'
     const int64_t most = (int64_t)g.S * g.D > (dw || db ? (int64_t)g.S * g.N : 0) ? (int64_t)g.S * g.D : (int64_t)g.S * g.N;
     const unsigned threads = join_threads(most);
+    const int64_t bytes = 2 * (int64_t)g.N * g.P * g.C * (int64_t)sizeof(T_);
+    const int backwards = bytes > kCache;
     by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
-        norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, kSums * g.Cs * sizeof(float), s>>>(x, dy, h, stats, w, b, part);
+        norm_bwd_sums_kernel<T_, V, ACT><<<blocks, kThreads, kSums * g.Cs * sizeof(float), s>>>(x, dy, h, stats, w, b, part, kept_from(bytes, blocks));
     });
     by_samples(g, g.G, threads, [&](const NormGeom& h, unsigned blocks) {
         const bool last = h.n0 + h.n1 == g.N && (dw || db);
         norm_bwd_join_kernel<<<blocks + (last ? g.C : 0), threads, 0, s>>>(part, h, w, coef, dw, db);
     });
-    const int backwards = (int64_t)g.N * g.P * g.C * (int64_t)sizeof(T_) > 128 << 20;         // beyond the last-level cache: what was read last first
     if (dx) by_samples(g, (int64_t)g.nslab * g.S, kThreads, [&](const NormGeom& h, unsigned blocks) {
         norm_bwd_apply_kernel<T_, V, ACT><<<blocks, kThreads, kFields * g.Cs * sizeof(float), s>>>(x, dy, h, stats, w, b, coef, dx, backwards);
     });

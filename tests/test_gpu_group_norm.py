@@ -312,6 +312,24 @@ def test_offsets_beyond_32_bits(dev):
         assert abs(y[n, channel, at[1], at[2]].double() - want) <= 2.0 ** -11 * abs(want) + 1e-4
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_beyond_the_last_level_cache(dev, dtype):
+    """More than 256 MB, where a pass streams most of its rows and the next begins at the end: every value of a few channels.  A
+    value passes through 32 rounds of a thread at most here, 10 levels and 6 joins: within the 64 of all the other sizes."""
+    from raft_amd import group_norm
+    N, C, H, W = 3, 48 if dtype == "fp32" else 104, 750, 683
+    g = torch.Generator(dev).manual_seed(3)
+    x, dy = [torch.randn(N, H, W, C, generator=g, device=dev).to(DTYPES[dtype]).movedim(-1, 1) for _ in range(2)]
+    w, b = [(1 + 0.3 * torch.randn(C, generator=g, device=dev)).requires_grad_(True) for _ in range(2)]
+    x.requires_grad_(True)
+    y = group_norm(x, C, w, b, activation="relu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    at = [0, 17, C - 1]
+    want = formula(x[:, at], w[at], b[at], len(at), 1e-5, "relu", dy[:, at])
+    for name, got, ref in zip(("y", "dx", "dw", "db"), (y[:, at], dx[:, at], dw[at], db[at]), want):
+        near(name, got, ref)
+
+
 def test_more_samples_than_a_launch_takes(dev):
     """2^24 + 100 samples of one row: a workgroup each would be 2^32 threads and more.  The channels' sums run over all samples: 64 u of
     the sum of sizes, and x's type is exact enough for d(y) = 1 to make d(bias) a count."""
