@@ -193,6 +193,12 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         buckets = self._ready()
         work = [(group, b) for group, of in zip(self.param_groups, buckets) for b in of if b.glue.collect(b.params)]
+        for group, b in work:               # options that went bad since, before anything is changed (one bucket's numbers: by the call itself)
+            lr = group["lr"]
+            if len(work) > 1 or torch.is_tensor(lr):
+                _options(group)
+                if torch.is_tensor(lr) and lr.is_cuda and lr.device != b.device:
+                    raise RuntimeError(f"lr is on {lr.device}, expected {b.device}")
         max_norm, partial, self.grad_norm = self.defaults["max_norm"], None, None
         if max_norm is not None:
             device = work[0][1].device if work else None
@@ -208,8 +214,6 @@ class AdamW(torch.optim.Optimizer):
         for group, b in work:
             lr, (b1, b2) = group["lr"], group["betas"]
             on_device = lr if torch.is_tensor(lr) and lr.is_cuda else None
-            if on_device is not None and on_device.device != b.device:
-                raise RuntimeError(f"lr is on {lr.device}, expected {b.device}")
             b.glue.step(b.bits, b.m, b.v, b.me, b.ve, b.steps, on_device, 0.0 if on_device is not None else float(lr), b1, b2, group["eps"],
                         group["weight_decay"], (group["seed"] + 7919 * b.index) & 0xFFFFFFFF, partial, max_norm or 0.0, self.grad_norm)
         return loss

@@ -459,6 +459,25 @@ def test_refusals(dev):
         AdamW([p], state_bits=8).packed_moments(torch.float64)
 
 
+@pytest.mark.parametrize("groups", [1, 2])
+@pytest.mark.parametrize("option", [{"lr": -1.0}, {"lr": "empty"}, {"lr": "half"}, {"betas": (0.9, 1.0)}, {"eps": -1.0}, {"weight_decay": float("nan")}], ids=str)
+def test_options_are_refused_before_anything_changes(dev, option, groups):
+    """An option that went bad after the construction, in the last group: the tensors of the others stay as they are too."""
+    from raft_amd import AdamW
+    ps = [torch.nn.Parameter(torch.ones(700, device=dev)) for _ in range(groups)]
+    opt = AdamW([{"params": [p]} for p in ps], max_norm=1.0)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    before = [p.detach().clone() for p in ps] + [opt.state[p][k].clone() for p in ps for k in ("step", "exp_avg", "exp_avg_sq")]
+    made = {"empty": torch.empty(0, device=dev), "half": torch.ones((), dtype=torch.float16, device=dev)}
+    opt.param_groups[-1].update({k: made.get(v, v) if isinstance(v, str) else v for k, v in option.items()})
+    with pytest.raises((ValueError, RuntimeError)):
+        opt.step()
+    after = [p.detach() for p in ps] + [opt.state[p][k] for p in ps for k in ("step", "exp_avg", "exp_avg_sq")]
+    assert all(torch.equal(a, b) for a, b in zip(after, before))
+
+
 def test_large_tensor(dev):
     """33 million values, the last of them a part of a tile."""
     from raft_amd import AdamW
