@@ -110,6 +110,7 @@ template <int V, typename S> __device__ __forceinline__ void reduce_columns(cons
 // the workgroup `kept` on, and streams the others.  Forward of 802 MB float32 with its reading order 406 us | 420 without both;
 // backward of 221 MB twice 176 | 184, of 802 MB twice 675 | 698, of 200 MB bfloat16 twice 168 | 176.
 // Kept 128 MB: 423, 181, 691, 172; 160: 420, 178, 685, 169; 192: 411, 177, 679, 166; 240: 404, 177, 670, 170.
+// Below 256 MB nothing is streamed: forward of 252 MB 124 us | 130, backward of 126 MB twice 104 | 117.
 constexpr int64_t kCache = 256LL << 20, kKept = 224LL << 20;
 
 template <bool ONCE, typename T_, int V>
@@ -122,7 +123,7 @@ __device__ __forceinline__ void load_next(Vec<T_, V>& v, const T_*& p, int64_t s
 // first of a summing launch's workgroups whose rows stay in the cache; bytes: of all that the pass reads
 static unsigned kept_from(int64_t bytes, unsigned blocks)
 {
-    return bytes <= kKept ? 0 : blocks - (unsigned)((double)blocks * kKept / (double)bytes);
+    return bytes <= kCache ? 0 : blocks - (unsigned)((double)blocks * kKept / (double)bytes);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
